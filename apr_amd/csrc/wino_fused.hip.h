@@ -26,42 +26,11 @@ namespace apr {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-#ifndef APR_WF_PK
-#define APR_WF_PK 1
-#endif
-// f32x2 add / subtract as ONE packed instruction (left to itself hipcc splits most of them into two v_add_f32)
-__device__ __forceinline__ f32x2 wf_add2(f32x2 a, f32x2 b)
-{
-#if APR_WF_PK
-    f32x2 r;
-    asm("v_pk_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-#else
-    return a + b;
-#endif
-}
-__device__ __forceinline__ f32x2 wf_sub2(f32x2 a, f32x2 b)
-{
-#if APR_WF_PK
-    f32x2 r;
-    asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-#else
-    return a - b;
-#endif
-}
-
+// f32x2 add / subtract, two scalar instructions: the packed-fp32 forms are off in every build (build.py says why)
+__device__ __forceinline__ f32x2 wf_add2(f32x2 a, f32x2 b) { return a + b; }
+__device__ __forceinline__ f32x2 wf_sub2(f32x2 a, f32x2 b) { return a - b; }
 // -a - b
-__device__ __forceinline__ f32x2 wf_nadd2(f32x2 a, f32x2 b)
-{
-#if APR_WF_PK
-    f32x2 r;
-    asm("v_pk_add_f32 %0, %1, %2 neg_lo:[1,1] neg_hi:[1,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-#else
-    return -a - b;
-#endif
-}
+__device__ __forceinline__ f32x2 wf_nadd2(f32x2 a, f32x2 b) { return -a - b; }
 // max(x, 0) as one instruction (fmaxf on a value out of inline asm costs a canonicalising v_max first); the sums
 // that reach it are never NaN-signalling, and v_max_f32 returns the other operand for a NaN like fmaxf
 __device__ __forceinline__ float wf_relu(float x)

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(512) void wino_fused8_f2(const float *__restrict__ 
     // the other wave's MFMAs, the other wave's own are exposed (wino_s2_fused.hip.h, tools/ws_stamps.py).  The U DMA is
     // therefore the work of waves 0-3 alone, a quarter of the image each in every step.
     // Stamps of the K step (-DW8_STAMPS, tools/ws_stamps.py): 4.8 k cycles against 4.1 k of MFMA issue.  The SIMDs of the
-    // step's store role are busy throughout: 48 MFMAs up to the barrier + 64 v_pk_add_f32 + 32 ds_write_b64 (their
+    // step's store role are busy throughout: 48 MFMAs up to the barrier + the transform's adds + 32 ds_write_b64 (their
     // VGPR transfer) + the DMA issue = 3.65 k cycles against 2.0-2.3 k on the SIMDs of the load role, which then wait at the
     // barrier: fp32 VALU and LDS stores take MFMA issue time one for one.  Measured and dropped: opposite roles on the two
     // waves of a SIMD (the transform work spread over all four SIMDs): the load-role wave takes the matrix pipe first, the
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(512) void wino_fused8_f2(const float *__restrict__ 
         //      The exchange runs through the buffers the last K step read, Vs[1] (pairs 0, 1) and Us[1] (pairs 2, 3).
         float *xw = wf_smem + (2 * (sub >> 1) + 1) * WF_POS + (((sub & 1) * 2 + ph) * 16) * 128 + lane * 2;          // what this wave hands over   [2 ep + column][lane][2]
         const float *xr = wf_smem + (2 * (sub >> 1) + 1) * WF_POS + (((sub & 1) * 2 + (ph ^ 1)) * 16) * 128 + lane * 2;   // what it receives
-        // two tile rows (e = 2 ep, 2 ep + 1: neighbouring accumulator registers) per packed instruction
+        // two tile rows (e = 2 ep, 2 ep + 1: neighbouring accumulator registers) at a time
         f32x2 keep[8][2];
         // PH_ is a literal: two straight-line copies, chosen once by the (scalar) parity
 #define W8_EPI_FIRST(PH_)                                                                                \

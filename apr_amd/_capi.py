@@ -14,6 +14,8 @@ FLAVOUR_GO, FLAVOUR_LIBROSA = 0, 1
 WARN_UNDERFLOW, WARN_OVERFLOW = 1, 2
 PROF_SLOTS = 48
 STATIC_MAX_WINDOWS = 64
+F32, F16, BF16 = 0, 1, 2          # element types of the label operators
+MAX_TOP = 32
 
 # every symbol include/apr.h declares (tests check the library exports all of them)
 SYMBOLS = (
@@ -26,6 +28,8 @@ SYMBOLS = (
     "apr_prepare_batch_device_static", "apr_engine_create_ex", "apr_sweep_plan", "apr_sweep_files_multi",
     "apr_bucket_hits_device", "apr_device_alloc", "apr_device_free", "apr_device_upload", "apr_device_download",
     "apr_gather_rows_device",
+    "apr_features_device", "apr_engine_num_features", "apr_label_logprobs_workspace", "apr_label_logprobs_device",
+    "apr_label_logprobs_backward_device", "apr_quantize_rows_device", "apr_linear_i8_device",
 )
 
 
@@ -135,6 +139,21 @@ def lib():
     L.apr_gather_rows_device.argtypes = [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.POINTER(C.c_size_t), C.c_int, C.POINTER(C.c_void_p),
                                          C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), vp, vp, vp]
     L.apr_gather_rows_device.restype = C.c_int
+    sz, dbl, ci = C.c_size_t, C.c_double, C.c_int
+    L.apr_features_device.argtypes = [vp, f32p, ci, f32p]
+    L.apr_features_device.restype = ci
+    L.apr_engine_num_features.argtypes = [vp]
+    L.apr_engine_num_features.restype = ci
+    L.apr_label_logprobs_workspace.argtypes = [sz, sz, ci]
+    L.apr_label_logprobs_workspace.restype = sz
+    L.apr_label_logprobs_device.argtypes = [vp, ci, vp, sz, sz, sz, dbl, vp, ci, vp, vp, vp, vp, vp, vp, sz]
+    L.apr_label_logprobs_device.restype = ci
+    L.apr_label_logprobs_backward_device.argtypes = [vp, ci, vp, sz, sz, sz, dbl, vp, vp, vp, vp, vp, vp, sz]
+    L.apr_label_logprobs_backward_device.restype = ci
+    L.apr_quantize_rows_device.argtypes = [vp, ci, vp, sz, sz, sz, vp, sz, vp]
+    L.apr_quantize_rows_device.restype = ci
+    L.apr_linear_i8_device.argtypes = [vp, vp, sz, vp, vp, sz, vp, vp, sz, sz, sz, ci, vp, sz]
+    L.apr_linear_i8_device.restype = ci
     L.apr_resample_taps.argtypes = [C.c_int, C.c_int, C.c_double, C.c_double, vp]
     L.apr_resample_taps.restype = C.c_int
     L.apr_upsample.argtypes = [vp, vp, C.c_size_t, C.c_int, vp, C.c_int, vp]

@@ -9,8 +9,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libapr_amd.so")
-SOURCES = ["engine.hip", "model_parse.cpp", "synth.cpp", "ingest.cpp"]
-HEADERS = ["conv.hip.h", "frontend.hip.h", "wino.hip.h", "wino4.hip.h", "wino4_fused.hip.h", "wino_fused.hip.h", "wino_fused8.hip.h", "wino_s2.hip.h", "wino_s2_fused.hip.h", "report.hip.h", "resample.hip.h", "conv12_fused.hip.h", "model_parse.h", os.path.join("..", "..", "include", "apr.h")]
+SOURCES = ["engine.hip", "operators.hip", "model_parse.cpp", "synth.cpp", "ingest.cpp"]
+HEADERS = ["conv.hip.h", "frontend.hip.h", "wino.hip.h", "wino4.hip.h", "wino4_fused.hip.h", "wino_fused.hip.h", "wino_fused8.hip.h", "wino_s2.hip.h", "wino_s2_fused.hip.h", "report.hip.h", "resample.hip.h", "conv12_fused.hip.h", "model_parse.h",
+           "engine_view.h", "element.hip.h", "logprob.hip.h", "rowquant.hip.h", "linear_i8.hip.h", os.path.join("..", "..", "include", "apr.h")]
 
 
 # Off in every build: hipcc -O3 forms v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32 from ordinary float code by itself, and some of their

@@ -584,4 +584,16 @@ __global__ __launch_bounds__(256) void head_kernel(const float *__restrict__ act
     if (logits && tid < C) logits[win * C + tid] = s_logit[tid];
 }
 
+// The first half of head_kernel: act [B][P][F] -> max over P -> feat [B][F].  One workgroup per window.
+__global__ __launch_bounds__(256) void pool_kernel(const float *__restrict__ act, int P, int F, float *__restrict__ feat)
+{
+    const long long win = blockIdx.x;
+    const float *a = act + win * (long long)P * F;
+    for (int c = threadIdx.x; c < F; c += 256) {
+        float m = a[c];
+        for (int p = 1; p < P; p++) m = fmaxf(m, a[(long long)p * F + c]);
+        feat[win * F + c] = m;
+    }
+}
+
 }  // namespace apr

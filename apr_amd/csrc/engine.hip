@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "../../include/apr.h"
+#include "engine_view.h"
 #include "conv.hip.h"
 #include "frontend.hip.h"
 #include "model_parse.h"
@@ -683,8 +684,9 @@ void launch_wino_gemm(apr_engine *e, const Layer &L, long long T)
                        L.d_u, L.d_b, e->d_M, 1, 1, L.cin, 1, 1, L.cout, (int)T, tiles_n);
 }
 
+// d_features: the pooled rows are written there, and the model's own head is not run
 int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int empty_class, float *d_logits, double *d_probs,
-            int32_t *d_label, uint8_t *d_match)
+            int32_t *d_label, uint8_t *d_match, float *d_features = nullptr)
 {
     if (e->layers.empty()) { e->err = "engine has no model (front-end only)"; return APR_ERR_NOMODEL; }
     const float *in = d_spec;
@@ -867,7 +869,9 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
         }
         in = out;
     }
-    {
+    if (d_features) {
+        hipLaunchKernelGGL(pool_kernel, dim3(batch), dim3(256), 0, e->stream, in, e->pool_pixels, e->features, d_features);
+    } else {
         ProfScope ps(e, e->head_slot, 2.0 * batch * e->features * e->n_classes,
                      4.0 * batch * e->pool_pixels * e->features);
         hipLaunchKernelGGL(head_kernel, dim3(batch), dim3(256), 0, e->stream, in, e->pool_pixels, e->features, e->d_wfc,
@@ -1016,6 +1020,28 @@ int check_engine(apr_engine *e)
 }
 
 }  // namespace
+
+namespace apr {
+
+bool engine_view(const apr_engine *e, EngineView &v) noexcept
+{
+    if (!e) return false;
+    v.device = e->device;
+    v.stream = e->stream;
+    v.n_cus = e->n_cus;
+    return true;
+}
+
+int engine_fail(apr_engine *e, int code, const char *text) noexcept
+{
+    try {
+        (e ? e->err : g_create_err) = text;
+    } catch (...) {   // no memory for the text: the code says enough
+    }
+    return code;
+}
+
+}  // namespace apr
 
 // ================================================================================================
 extern "C" {
@@ -1289,6 +1315,21 @@ int apr_infer_device(apr_engine *e, const float *d_spec, int batch, float *d_log
     for (int b0 = 0; b0 < batch; b0 += e->max_batch) {
         const int nb = std::min(e->max_batch, batch - b0);
         if ((rc = run_cnn(e, d_spec + (size_t)b0 * APR_SPEC_ELEMS, nb, 0.0, -1, d_logits + (size_t)b0 * e->n_classes, nullptr, nullptr, nullptr))) return rc;
+    }
+    return APR_OK;
+}
+
+int apr_engine_num_features(const apr_engine *e) { return e && !e->layers.empty() ? e->features : 0; }
+
+int apr_features_device(apr_engine *e, const float *d_spec, int batch, float *d_features)
+{
+    int rc = check_engine(e);
+    if (rc) return rc;
+    if (e->layers.empty()) { e->err = "engine has no model (front-end only)"; return APR_ERR_NOMODEL; }
+    if (batch < 0 || (batch && (!d_spec || !d_features))) { e->err = "apr_features_device: bad argument"; return APR_ERR_INVALID; }
+    for (int b0 = 0; b0 < batch; b0 += e->max_batch) {
+        const int nb = std::min(e->max_batch, batch - b0);
+        if ((rc = run_cnn(e, d_spec + (size_t)b0 * APR_SPEC_ELEMS, nb, 0.0, -1, nullptr, nullptr, nullptr, nullptr, d_features + (size_t)b0 * e->features))) return rc;
     }
     return APR_OK;
 }

@@ -1,0 +1,40 @@
+// engine_view.h -- what a translation unit beside engine.hip needs of an engine: its GPU, its stream, and where its error text goes.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../include/apr.h"
+
+namespace apr {
+
+struct EngineView {
+    int device;
+    hipStream_t stream;
+    int n_cus;
+};
+// false for a null handle
+bool engine_view(const apr_engine *e, EngineView &v) noexcept;
+// Keeps `text` as the engine's last error (this thread's, for a null handle) and returns `code`.
+int engine_fail(apr_engine *e, int code, const char *text) noexcept;
+
+// Makes a device current for a scope and puts the caller's back: torch and other libraries in the process go by the current device.
+class DeviceScope {
+    int before_ = -1;
+    bool ok_ = false;
+
+public:
+    explicit DeviceScope(int device) noexcept
+    {
+        if (hipGetDevice(&before_) != hipSuccess) { before_ = -1; return; }
+        ok_ = before_ == device || hipSetDevice(device) == hipSuccess;
+        if (before_ == device) before_ = -1;
+    }
+    ~DeviceScope()
+    {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+    bool ok() const noexcept { return ok_; }
+};
+
+}  // namespace apr

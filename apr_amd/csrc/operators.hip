@@ -1,0 +1,174 @@
+// operators.hip -- C ABI of the operators behind a label head (include/apr.h): argument checks and launches.
+//
+// Every entry checks its arguments before it looks at the engine, so that a bad call is an error code on a host without a GPU too,
+// allocates nothing, and issues kernels only, on the engine's stream: it may be captured into a graph.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <type_traits>
+
+#include "../../include/apr.h"
+#include "engine_view.h"
+#include "linear_i8.hip.h"
+#include "logprob.hip.h"
+#include "rowquant.hip.h"
+
+using namespace apr;
+
+namespace {
+
+constexpr size_t kMostRows = 0x7FFFFFFF, kMostStride = (size_t)1 << 40;
+constexpr unsigned kMostBlocks = 1u << 20;   // grids stride over their rows beyond that
+
+size_t element_size(int dtype) { return dtype == APR_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == APR_F32 || dtype == APR_F16 || dtype == APR_BF16; }
+bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+int refuse(apr_engine *e, const char *entry, const char *why)
+{
+    char text[256];
+    snprintf(text, sizeof text, "%s: bad argument (%s)", entry, why);
+    return engine_fail(e, APR_ERR_INVALID, text);
+}
+
+// the launches of one entry: on the engine's GPU and stream, the caller's device back afterwards
+template <class F>
+int on_engine(apr_engine *e, const char *entry, F launch)
+{
+    EngineView v;
+    char text[256];
+    if (!engine_view(e, v)) {
+        snprintf(text, sizeof text, "%s: null engine", entry);
+        return engine_fail(e, APR_ERR_INVALID, text);
+    }
+    DeviceScope scope(v.device);
+    if (!scope.ok()) return engine_fail(e, APR_ERR_DEVICE, "hipSetDevice failed");
+    launch(v);
+    const hipError_t r = hipGetLastError();
+    if (r == hipSuccess) return APR_OK;
+    snprintf(text, sizeof text, "%s: %s", entry, hipGetErrorString(r));
+    return engine_fail(e, APR_ERR_DEVICE, text);
+}
+
+// calls f with a null pointer of the element type
+template <class F>
+void with_type(int dtype, F f)
+{
+    if (dtype == APR_F32) f((float *)nullptr);
+    else if (dtype == APR_F16) f((f16_t *)nullptr);
+    else f((bf16_t *)nullptr);
+}
+#define APR_TYPE_OF(p) std::remove_pointer_t<decltype(p)>
+
+}  // namespace
+
+extern "C" {
+
+size_t apr_label_logprobs_workspace(size_t n, size_t n_labels, int top)
+{
+    (void)n; (void)n_labels; (void)top;
+    return 0;
+}
+
+int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld, double scale,
+                              const int32_t *d_target, int top, float *d_logprob, float *d_entropy, float *d_stat, int32_t *d_top_label,
+                              float *d_top_logprob, void *d_work, size_t work_bytes)
+{
+    const char *me = "apr_label_logprobs_device";
+    if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
+    if (n > kMostRows || n_labels < 1 || n_labels > kMostRows) return refuse(e, me, "1 <= n_labels < 2^31, n < 2^31");
+    if (ld < n_labels || ld > kMostStride) return refuse(e, me, "ld is at least n_labels");
+    if (!(scale > 0.0) || !std::isfinite((float)scale) || (float)scale == 0.0f) return refuse(e, me, "scale is positive and finite");
+    if (top < 0 || top > APR_MAX_TOP) return refuse(e, me, "0 <= top <= APR_MAX_TOP");
+    if (d_logprob && !d_target) return refuse(e, me, "d_logprob needs d_target");
+    if (top == 0 && (d_top_label || d_top_logprob)) d_top_label = nullptr, d_top_logprob = nullptr;
+    if (!d_top_label && !d_top_logprob) top = 0;
+    if (!n) return on_engine(e, me, [](const EngineView &) {});
+    if (!d_logits) return refuse(e, me, "null d_logits");
+    if (!aligned(d_logits, element_size(dtype)) || !aligned(d_target, 4) || !aligned(d_logprob, 4) || !aligned(d_entropy, 4) || !aligned(d_stat, 4) ||
+        !aligned(d_top_label, 4) || !aligned(d_top_logprob, 4))
+        return refuse(e, me, "pointers are aligned to their element");
+    const size_t need = apr_label_logprobs_workspace(n, n_labels, top);
+    if (need && (!d_work || work_bytes < need || !aligned(d_work, 16))) return refuse(e, me, "d_work holds apr_label_logprobs_workspace bytes, 16-aligned");
+    LogprobArgs a;
+    a.x = d_logits; a.n = n; a.ld = ld; a.n_labels = (unsigned)n_labels; a.scale = (float)scale; a.target = d_target; a.top = top;
+    a.logprob = d_logprob; a.entropy = d_entropy; a.stat = d_stat; a.top_label = d_top_label; a.top_logprob = d_top_logprob;
+    return on_engine(e, me, [&](const EngineView &v) {
+        with_type(dtype, [&](auto *p) {
+            hipLaunchKernelGGL(logprob_rows_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(256), 0, v.stream, a);
+        });
+    });
+}
+
+int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld, double scale,
+                                       const int32_t *d_target, const float *d_stat, const float *d_entropy, const float *d_g_logprob,
+                                       const float *d_g_entropy, void *d_grad, size_t ld_grad)
+{
+    const char *me = "apr_label_logprobs_backward_device";
+    if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
+    if (n > kMostRows || n_labels < 1 || n_labels > kMostRows) return refuse(e, me, "1 <= n_labels < 2^31, n < 2^31");
+    if (ld < n_labels || ld > kMostStride || ld_grad < n_labels || ld_grad > kMostStride) return refuse(e, me, "ld and ld_grad are at least n_labels");
+    if (!(scale > 0.0) || !std::isfinite((float)scale) || (float)scale == 0.0f) return refuse(e, me, "scale is positive and finite");
+    if (d_g_logprob && !d_target) return refuse(e, me, "d_g_logprob needs d_target");
+    if (d_g_entropy && !d_entropy) return refuse(e, me, "d_g_entropy needs d_entropy");
+    if (!n) return on_engine(e, me, [](const EngineView &) {});
+    if (!d_logits || !d_stat || !d_grad) return refuse(e, me, "null d_logits, d_stat or d_grad");
+    if (!aligned(d_logits, element_size(dtype)) || !aligned(d_grad, element_size(dtype)) || !aligned(d_target, 4) || !aligned(d_stat, 4) ||
+        !aligned(d_entropy, 4) || !aligned(d_g_logprob, 4) || !aligned(d_g_entropy, 4))
+        return refuse(e, me, "pointers are aligned to their element");
+    if (d_grad == d_logits && ld_grad != ld) return refuse(e, me, "a gradient in the place of the scores has their stride");
+    LogprobGradArgs a;
+    a.x = d_logits; a.grad = d_grad; a.n = n; a.ld = ld; a.ld_grad = ld_grad; a.n_labels = (unsigned)n_labels; a.scale = (float)scale;
+    a.target = d_target; a.stat = d_stat; a.entropy = d_entropy; a.g_logprob = d_g_logprob; a.g_entropy = d_g_entropy;
+    return on_engine(e, me, [&](const EngineView &v) {
+        with_type(dtype, [&](auto *p) {
+            hipLaunchKernelGGL(logprob_grad_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(256), 0, v.stream, a);
+        });
+    });
+}
+
+int apr_quantize_rows_device(apr_engine *e, int dtype, const void *d_x, size_t n, size_t k, size_t ld, int8_t *d_q, size_t ld_q, float *d_scale)
+{
+    const char *me = "apr_quantize_rows_device";
+    if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
+    if (n > kMostRows || k < 1 || k > kMostRows) return refuse(e, me, "1 <= k < 2^31, n < 2^31");
+    if (ld < k || ld > kMostStride || ld_q < k || ld_q > kMostStride) return refuse(e, me, "ld and ld_q are at least k");
+    if (!n) return on_engine(e, me, [](const EngineView &) {});
+    if (!d_x || !d_q || !d_scale) return refuse(e, me, "null pointer");
+    if (!aligned(d_x, element_size(dtype)) || !aligned(d_scale, 4)) return refuse(e, me, "pointers are aligned to their element");
+    RowQuantArgs a;
+    a.x = d_x; a.q = d_q; a.scale = d_scale; a.n = n; a.ld = ld; a.ld_q = ld_q; a.k = (unsigned)k;
+    return on_engine(e, me, [&](const EngineView &v) {
+        with_type(dtype, [&](auto *p) {
+            hipLaunchKernelGGL(rowquant_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(256), 0, v.stream, a);
+        });
+    });
+}
+
+int apr_linear_i8_device(apr_engine *e, const int8_t *d_x, size_t ld_x, const float *d_x_scale, const int8_t *d_w, size_t ld_w,
+                         const float *d_w_scale, const float *d_bias, size_t m, size_t n, size_t k, int dtype, void *d_out, size_t ld_out)
+{
+    const char *me = "apr_linear_i8_device";
+    if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
+    if (m > APR_LINEAR_MAX_ROWS || n > APR_LINEAR_MAX_ROWS) return refuse(e, me, "m and n are at most APR_LINEAR_MAX_ROWS");
+    if (k < 1 || k > APR_LINEAR_MAX_K) return refuse(e, me, "1 <= k <= APR_LINEAR_MAX_K: the sum has 32 bits");
+    if (ld_x < k || ld_x > kMostStride || ld_w < k || ld_w > kMostStride || ld_out < n || ld_out > kMostStride)
+        return refuse(e, me, "ld_x and ld_w are at least k, ld_out at least n");
+    if (!m || !n) return on_engine(e, me, [](const EngineView &) {});
+    if (!d_x || !d_w || !d_x_scale || !d_w_scale || !d_out) return refuse(e, me, "null pointer");
+    if (!aligned(d_out, element_size(dtype)) || !aligned(d_x_scale, 4) || !aligned(d_w_scale, 4) || !aligned(d_bias, 4))
+        return refuse(e, me, "pointers are aligned to their element");
+    LinearI8Args a;
+    a.x = d_x; a.w = d_w; a.x_scale = d_x_scale; a.w_scale = d_w_scale; a.bias = d_bias; a.out = d_out;
+    a.ld_x = ld_x; a.ld_w = ld_w; a.ld_out = ld_out; a.m = (unsigned)m; a.n = (unsigned)n; a.k = (unsigned)k;
+    const unsigned long long tiles = ((m + 63) / 64) * ((n + 63) / 64);
+    return on_engine(e, me, [&](const EngineView &v) {
+        with_type(dtype, [&](auto *p) {
+            hipLaunchKernelGGL(linear_i8_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<unsigned long long>(tiles, kMostBlocks)), dim3(256), 0, v.stream, a);
+        });
+    });
+}
+
+}  // extern "C"

@@ -111,6 +111,24 @@ def _as_u8(buf) -> np.ndarray:
     return np.frombuffer(buf, dtype=np.uint8)
 
 
+_I8 = 3                              # int8, beside the _capi.F32 / F16 / BF16 of the C ABI
+_ELEMENT_TYPES = {"torch.float32": _capi.F32, "torch.float16": _capi.F16, "torch.bfloat16": _capi.BF16, "torch.int8": _I8}
+
+
+def _element_type(t) -> int:
+    return _ELEMENT_TYPES.get(str(t.dtype), -1)
+
+
+def torch_stream(engine: "Engine"):
+    """The engine's stream for torch: work queued under ``torch.cuda.stream(torch_stream(engine))`` runs in order with the
+    engine's calls, so nothing has to be waited for between the two."""
+    import torch
+    s = getattr(engine, "_torch_stream", None)
+    if s is None:
+        s = engine._torch_stream = torch.cuda.ExternalStream(engine._lib.apr_engine_stream(engine._h), device=engine.device)
+    return s
+
+
 class Engine:
     """apr_engine handle (include/apr.h).  ``model_bytes=None`` gives a front-end-only engine."""
 
@@ -325,6 +343,101 @@ class Engine:
             msg = (lib.apr_last_error(engines[root]._h) if 0 <= root < n else b"") or lib.apr_last_error(None) or b""
             raise AprError(rc, msg.decode())
 
+    # ---- operators behind a label head (device-resident: torch tensors on this engine's GPU, or addresses) ----
+    def _matrix(self, name: str, a, rows: int, cols: int, ld: Optional[int], dtype: Optional[int] = None, types=(0, 1, 2)):
+        """(address, row stride, element type) of a [rows, cols] operand.  A tensor speaks for itself and is checked; for an
+        address the caller gives ``ld`` (default: cols) and ``dtype``."""
+        if isinstance(a, int):
+            return a, cols if ld is None else ld, types[0] if dtype is None else dtype
+        if not hasattr(a, "data_ptr"):
+            raise TypeError(f"{name}: a torch tensor on the engine's GPU or a device address, not {type(a).__name__}")
+        code = _element_type(a)
+        if code not in types or (dtype is not None and code != dtype):
+            raise ValueError(f"{name}: {a.dtype} is not the element type this operand has")
+        if not a.is_cuda or a.device.index != self.device:
+            raise ValueError(f"{name} is on {a.device}, the engine on GPU {self.device}")
+        if a.dim() == 2:
+            if a.shape[0] < rows or a.shape[1] < cols:
+                raise ValueError(f"{name}: {tuple(a.shape)} does not hold {rows} x {cols}")
+            if cols > 1 and a.stride(1) != 1:
+                raise ValueError(f"{name}: the elements of a row have to be contiguous")
+            own = a.stride(0) if rows > 1 else max(a.shape[1], cols)
+            if ld is not None and ld != own and rows > 1:
+                raise ValueError(f"{name}: its rows are {own} elements apart, not {ld}")
+            return a.data_ptr(), own, code
+        ld = cols if ld is None else ld
+        if not a.is_contiguous() or (rows and a.numel() < (rows - 1) * ld + cols):
+            raise ValueError(f"{name}: {tuple(a.shape)} does not hold {rows} x {cols} at a row stride of {ld}")
+        return a.data_ptr(), ld, code
+
+    def _vector(self, name: str, a, count: int, kind: str) -> int:
+        """address of `count` contiguous float32 / int32 values (0 for None)"""
+        if a is None:
+            return 0
+        if isinstance(a, int):
+            return a
+        if not hasattr(a, "data_ptr"):
+            raise TypeError(f"{name}: a torch tensor on the engine's GPU or a device address, not {type(a).__name__}")
+        if str(a.dtype) != "torch." + kind or not a.is_contiguous() or a.numel() < count:
+            raise ValueError(f"{name}: {count} contiguous {kind} values are needed, not {tuple(a.shape)} of {a.dtype}")
+        if not a.is_cuda or a.device.index != self.device:
+            raise ValueError(f"{name} is on {a.device}, the engine on GPU {self.device}")
+        return a.data_ptr()
+
+    def label_logprobs_workspace(self, n: int, n_labels: int, top: int = 0) -> int:
+        """apr_label_logprobs_workspace: bytes of ``d_work`` a call of these sizes needs."""
+        return int(self._lib.apr_label_logprobs_workspace(n, n_labels, top))
+
+    def label_logprobs_device(self, d_logits, n: int, n_labels: int, d_target=None, top: int = 0, d_logprob=None, d_entropy=None,
+                              d_stat=None, d_top_label=None, d_top_logprob=None, d_work=None, scale: float = 1.0,
+                              ld: Optional[int] = None, dtype: Optional[int] = None, work_bytes: Optional[int] = None) -> None:
+        """apr_label_logprobs_device: log probability of each row's label, entropy, the `top` best labels with theirs."""
+        x, ld, code = self._matrix("d_logits", d_logits, n, n_labels, ld, dtype)
+        if work_bytes is None:
+            work_bytes = d_work.numel() * d_work.element_size() if hasattr(d_work, "numel") else 0
+        self._chk(self._lib.apr_label_logprobs_device(
+            self._h, code, x, n, n_labels, ld, scale, self._vector("d_target", d_target, n, "int32"), top,
+            self._vector("d_logprob", d_logprob, n, "float32"), self._vector("d_entropy", d_entropy, n, "float32"),
+            self._vector("d_stat", d_stat, 2 * n, "float32"), self._vector("d_top_label", d_top_label, n * top, "int32"),
+            self._vector("d_top_logprob", d_top_logprob, n * top, "float32"), _addr(d_work), work_bytes))
+
+    def label_logprobs_backward_device(self, d_logits, n: int, n_labels: int, d_target, d_stat, d_grad, d_g_logprob=None,
+                                       d_entropy=None, d_g_entropy=None, scale: float = 1.0, ld: Optional[int] = None,
+                                       ld_grad: Optional[int] = None, dtype: Optional[int] = None) -> None:
+        """apr_label_logprobs_backward_device: gradient of sum(g_logprob * logprob + g_entropy * entropy) for the logits."""
+        x, ld, code = self._matrix("d_logits", d_logits, n, n_labels, ld, dtype)
+        grad, ld_grad, _ = self._matrix("d_grad", d_grad, n, n_labels, ld_grad, code)
+        self._chk(self._lib.apr_label_logprobs_backward_device(
+            self._h, code, x, n, n_labels, ld, scale, self._vector("d_target", d_target, n, "int32"),
+            self._vector("d_stat", d_stat, 2 * n, "float32"), self._vector("d_entropy", d_entropy, n, "float32"),
+            self._vector("d_g_logprob", d_g_logprob, n, "float32"), self._vector("d_g_entropy", d_g_entropy, n, "float32"), grad, ld_grad))
+
+    def quantize_rows_device(self, d_x, n: int, k: int, d_q, d_scale, ld: Optional[int] = None, ld_q: Optional[int] = None,
+                             dtype: Optional[int] = None) -> None:
+        """apr_quantize_rows_device: rows as int8 with one float32 scale each."""
+        x, ld, code = self._matrix("d_x", d_x, n, k, ld, dtype)
+        q, ld_q, _ = self._matrix("d_q", d_q, n, k, ld_q, None, (_I8,))
+        self._chk(self._lib.apr_quantize_rows_device(self._h, code, x, n, k, ld, q, ld_q, self._vector("d_scale", d_scale, n, "float32")))
+
+    def linear_i8_device(self, d_x, d_x_scale, d_w, d_w_scale, m: int, n: int, k: int, d_out, d_bias=None, ld_x: Optional[int] = None,
+                         ld_w: Optional[int] = None, ld_out: Optional[int] = None, dtype: Optional[int] = None) -> None:
+        """apr_linear_i8_device: [m, k] int8 times [n, k] int8 transposed, a scale for each row of both, -> [m, n]."""
+        x, ld_x, _ = self._matrix("d_x", d_x, m, k, ld_x, None, (_I8,))
+        w, ld_w, _ = self._matrix("d_w", d_w, n, k, ld_w, None, (_I8,))
+        out, ld_out, code = self._matrix("d_out", d_out, m, n, ld_out, dtype)
+        self._chk(self._lib.apr_linear_i8_device(
+            self._h, x, ld_x, self._vector("d_x_scale", d_x_scale, m, "float32"), w, ld_w, self._vector("d_w_scale", d_w_scale, n, "float32"),
+            self._vector("d_bias", d_bias, n, "float32"), m, n, k, code, out, ld_out))
+
+    @property
+    def num_features(self) -> int:
+        """width of the rows ``features_device`` writes (0 for a front-end-only engine)"""
+        return self._lib.apr_engine_num_features(self._h)
+
+    def features_device(self, d_spec, batch: int, d_features) -> None:
+        """apr_features_device: the pooled rows that the CNN's own head reads, for a head of one's own."""
+        self._chk(self._lib.apr_features_device(self._h, _addr(d_spec), batch, _addr(d_features)))
+
     def infer_device(self, d_spec, batch: int, d_logits) -> None:
         self._chk(self._lib.apr_infer_device(self._h, _addr(d_spec), batch, _addr(d_logits)))
 
@@ -358,6 +471,128 @@ def windows_in(n_bytes: int, stride: int = BytesPerSecond) -> int:
     if n_bytes <= stride:
         return 0
     return len(range(0, n_bytes - stride, stride))
+
+
+def _release(engine: Engine, addresses: List[int]) -> None:
+    while addresses:
+        engine.device_free(addresses.pop())
+
+
+class LabelHead:
+    """A list of labels of any length over the features of an engine's CNN: a Linear with 8-bit weights (one scale for each label;
+    the features are quantised with one scale for each window) and what it answers -- the log probability of a given label, the
+    entropy of the answer, the best alternatives.  The CNN's own head stays as it is: this one stands beside it, so that one pass of
+    the convolutions serves a longer list (the reference has one head a model, at most 64 labels here).
+
+    weight [labels][features] and bias [labels] as in torch.nn.Linear; scale is 1 / temperature.  Close it before its engine."""
+
+    def __init__(self, engine: Engine, weight, bias=None, scale: float = 1.0, max_rows: int = 1024):
+        w = np.ascontiguousarray(weight, np.float32)
+        f = engine.num_features
+        if w.ndim != 2 or w.shape[0] < 1 or w.shape[1] != f or f == 0:
+            raise ValueError(f"weight is [labels, {f}], not {w.shape}")
+        b = None if bias is None else np.ascontiguousarray(bias, np.float32)
+        if b is not None and b.shape != (w.shape[0],):
+            raise ValueError(f"bias is [{w.shape[0]}], not {b.shape}")
+        if max_rows < 1:
+            raise ValueError("max_rows is at least 1")
+        self.engine, self.labels, self.scale, self.max_rows = engine, w.shape[0], float(scale), max_rows
+        self._f, self._ld = f, -(-f // 16) * 16
+        self._own: List[int] = []
+        self._fin = weakref.finalize(self, _release, engine, self._own)
+        n, c = max_rows, self.labels
+        self._w = self._alloc(c * self._ld)
+        self._w_scale = self._alloc(4 * c)
+        self._bias = None
+        if b is not None:
+            self._bias = self._alloc(4 * c)
+            engine.device_upload(self._bias, b)
+        real = self._alloc(w.nbytes)
+        engine.device_upload(real, w)
+        engine.quantize_rows_device(real, c, f, self._w, self._w_scale, ld_q=self._ld)
+        engine.sync()
+        self._own.remove(real)
+        engine.device_free(real)
+        self._spec = self._alloc(n * Nmels * SpectrogramFrames * 4)
+        self._feat = self._alloc(n * f * 4)
+        self._q = self._alloc(n * self._ld)
+        self._q_scale = self._alloc(n * 4)
+        self._logits = self._alloc(n * c * 4)
+        self._small = {k: self._alloc(n * size * 4) for k, size in
+                       dict(target=1, logprob=1, entropy=1, stat=2, g=1, top_label=_capi.MAX_TOP, top_logprob=_capi.MAX_TOP).items()}
+        self._work_bytes = max(engine.label_logprobs_workspace(r, c, _capi.MAX_TOP) for r in range(1, n + 1))
+        self._work = self._alloc(self._work_bytes) if self._work_bytes else None
+
+    def _alloc(self, nbytes: int) -> int:
+        p = self.engine.device_alloc(nbytes)
+        self._own.append(p)
+        return p
+
+    def close(self) -> None:
+        self._fin()
+
+    def _forward(self, spec: np.ndarray, target: Optional[np.ndarray], top: int) -> None:
+        """a pass of at most max_rows windows, queued on the engine's stream"""
+        e, n, m = self.engine, len(spec), self._small
+        e.device_upload(self._spec, spec)
+        if target is not None:
+            e.device_upload(m["target"], target)
+        e.features_device(self._spec, n, self._feat)
+        e.quantize_rows_device(self._feat, n, self._f, self._q, self._q_scale, ld_q=self._ld)
+        e.linear_i8_device(self._q, self._q_scale, self._w, self._w_scale, n, self.labels, self._f, self._logits, d_bias=self._bias,
+                           ld_x=self._ld, ld_w=self._ld)
+        e.label_logprobs_device(self._logits, n, self.labels, d_target=m["target"] if target is not None else None, top=top,
+                                d_logprob=m["logprob"] if target is not None else None, d_entropy=m["entropy"], d_stat=m["stat"],
+                                d_top_label=m["top_label"], d_top_logprob=m["top_logprob"], d_work=self._work,
+                                work_bytes=self._work_bytes, scale=self.scale)
+
+    def _arguments(self, spec, target):
+        s = np.ascontiguousarray(spec, np.float32).reshape(-1, Nmels, SpectrogramFrames)
+        if target is None:
+            return s, None
+        t = np.ascontiguousarray(target, np.int32)
+        if t.shape != (len(s),):
+            raise ValueError(f"target is [{len(s)}], not {t.shape}")
+        return s, t
+
+    def score(self, spec, target=None, top: int = 5) -> dict:
+        """Prepared spectrograms [n][128][188] -> dict(entropy [n], top_label [n, top], top_logprob [n, top], and with
+        target [n]: logprob [n])."""
+        s, t = self._arguments(spec, target)
+        if not 0 <= top <= _capi.MAX_TOP:
+            raise ValueError(f"top is 0 to {_capi.MAX_TOP}")
+        n = len(s)
+        out = dict(entropy=np.empty(n, np.float32), top_label=np.empty((n, top), np.int32), top_logprob=np.empty((n, top), np.float32))
+        if t is not None:
+            out["logprob"] = np.empty(n, np.float32)
+        for a in range(0, n, self.max_rows):
+            z = min(n, a + self.max_rows)
+            self._forward(s[a:z], None if t is None else t[a:z], top)
+            for k, v in out.items():
+                self.engine.device_download(self._small[k], v[a:z])
+        return out
+
+    def loss(self, spec, target) -> dict:
+        """Cross entropy of the labels, averaged over the windows that have one (0 <= target < labels), with what a training step
+        of the head needs -> dict(loss, d_logits [n, labels], features [n, features]): the weight's gradient is
+        d_logits.T @ features, the bias's d_logits.sum(0)."""
+        s, t = self._arguments(spec, target)
+        if t is None:
+            raise ValueError("a loss needs targets")
+        n, count = len(s), int(((t >= 0) & (t < self.labels)).sum())
+        logprob = np.empty(n, np.float32)
+        grad, feat = np.empty((n, self.labels), np.float32), np.empty((n, self._f), np.float32)
+        e, m = self.engine, self._small
+        for a in range(0, n, self.max_rows):
+            z = min(n, a + self.max_rows)
+            self._forward(s[a:z], t[a:z], 0)
+            e.device_upload(m["g"], np.full(z - a, -1.0 / max(count, 1), np.float32))
+            e.device_download(m["logprob"], logprob[a:z])
+            e.label_logprobs_backward_device(self._logits, z - a, self.labels, m["target"], m["stat"], self._logits, d_g_logprob=m["g"],
+                                             scale=self.scale)
+            e.device_download(self._logits, grad[a:z])
+            e.device_download(self._feat, feat[a:z])
+        return dict(loss=-float(logprob.astype(np.float64).sum()) / max(count, 1), d_logits=grad, features=feat)
 
 
 # ------------------------------------------------------------------------------------------

@@ -35,6 +35,14 @@ extern "C" {
 #define APR_SPEC_ELEMS         (APR_NMELS * APR_SPECTROGRAM_FRAMES)
 #define APR_MAX_CLASSES        64
 
+/* element types of the label operators (apr_label_logprobs_device ... apr_linear_i8_device) */
+#define APR_F32  0
+#define APR_F16  1
+#define APR_BF16 2
+#define APR_MAX_TOP         32          /* best alternatives a row                  */
+#define APR_LINEAR_MAX_K    131071      /* k * 128 * 128 fits 32 bits               */
+#define APR_LINEAR_MAX_ROWS 16777216    /* rows of x, rows of w                     */
+
 /* error codes */
 #define APR_OK            0
 #define APR_ERR_INVALID  -1   /* bad argument                                   */
@@ -300,6 +308,75 @@ int apr_bucket_hits(const int32_t *label, const uint8_t *match, size_t n_windows
  * every byte of d_hits is written; n_classes <= APR_MAX_CLASSES.  Asynchronous on the engine's stream. */
 int apr_bucket_hits_device(apr_engine *e, const int32_t *d_label, const uint8_t *d_match, size_t n_windows, int n_classes,
                            size_t windows_per_bucket, uint8_t *d_hits);
+
+/*
+ * The row the CNN's own Linear reads: 12 conv layers + global max-pool of `batch` spectrograms -> d_features
+ * [batch][apr_engine_num_features] f32 (AdaptiveMaxPool2d(1) + Flatten of ai/model.py:105-110; Dropout is the identity at
+ * inference).  What a second head over the same CNN is trained on and answers from.  Asynchronous on the engine's stream.
+ */
+int apr_features_device(apr_engine *e, const float *d_spec, int batch, float *d_features);
+int apr_engine_num_features(const apr_engine *e);   /* 0 for a front-end-only engine */
+
+/*
+ * ---- operators behind a label head: any number of labels, any source of the scores ----
+ * No counterpart in the reference, whose only head is the CNN's (at most APR_MAX_CLASSES classes, f64 softmax, best label).
+ * They chain as  features -> apr_quantize_rows_device -> apr_linear_i8_device -> apr_label_logprobs_device
+ * [-> apr_label_logprobs_backward_device]; apr_amd/model.py: LabelHead is that chain over an engine's features.
+ * All pointers are device pointers on the engine's GPU, aligned to their element; a front-end-only engine will do.
+ * Asynchronous on the engine's stream (inputs that another stream is still writing have to be waited for first:
+ * apr_engine_stream); nothing is allocated and only kernels are launched, so a call may be captured into a graph.
+ * The current device of the calling thread is left as it was.  Matrices are row-major with a row stride `ld` in elements;
+ * what lies between the rows' ends is neither used nor written.  Zero rows are a no-op.
+ */
+
+/*
+ * Log probabilities of given labels over rows of scores (APR_F32 / APR_F16 / APR_BF16), with entropy and best alternatives:
+ * p = softmax(scale * logits) of each row, scale > 0 (1 / temperature); all sums in 32 bits, relative to the row's maximum.
+ *   d_target      [n]       label whose log probability is wanted; one outside [0, n_labels) names none: logprob 0
+ *   d_logprob     [n]       log p[target]                              (needs d_target)
+ *   d_entropy     [n]       -sum p log p, in nats
+ *   d_stat        [n][2]    the row's largest logit, and log sum exp(scale * (logit - largest)): log-sum-exp =
+ *                           scale * stat[0] + stat[1]; what the backward call starts from
+ *   d_top_label   [n][top]  the `top` labels of largest score, best first, equal scores lowest label first
+ *   d_top_logprob [n][top]  their log probabilities
+ * Any output may be NULL.  A logit of -inf rules its label out: p = 0, never an alternative; places that no label fills hold -1 and
+ * -inf.  A row with every label ruled out: logprob -inf, entropy 0, stat (-inf, -inf).  A row that holds NaN or +inf: NaN everywhere,
+ * top_label -1.  1 <= n_labels < 2^31, 0 <= top <= APR_MAX_TOP.
+ *   d_work        scratch of apr_label_logprobs_workspace(n, n_labels, top) bytes, 16-byte aligned (0 bytes: NULL will do).  A
+ *                 graph keeps its address: two calls that may run at the same time need two.
+ */
+size_t apr_label_logprobs_workspace(size_t n, size_t n_labels, int top);
+int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld, double scale,
+                              const int32_t *d_target, int top, float *d_logprob, float *d_entropy, float *d_stat,
+                              int32_t *d_top_label, float *d_top_logprob, void *d_work, size_t work_bytes);
+
+/*
+ * Gradient of sum_i g_logprob[i] * logprob[i] + g_entropy[i] * entropy[i] with respect to the logits, in the logits' type (one
+ * rounding).  d_stat and d_entropy are what the forward call wrote for these logits and this scale.  d_g_logprob (needs d_target)
+ * or d_g_entropy (needs d_entropy) may be NULL: zero.  Cross entropy averaged over n rows: g_logprob = -1 / n.  A target outside
+ * [0, n_labels) has no gradient, a row with every label ruled out neither; a row of NaN gives NaN.  d_grad may be d_logits.
+ */
+int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld,
+                                       double scale, const int32_t *d_target, const float *d_stat, const float *d_entropy,
+                                       const float *d_g_logprob, const float *d_g_entropy, void *d_grad, size_t ld_grad);
+
+/*
+ * Rows as 8-bit whole numbers with one scale each: d_scale[i] = max|x_i| / 127, d_q[i][j] = 127 x / max|x_i| rounded to nearest even
+ * (the exact quotient), so x ~ q * scale.  The rows are windows (a scale for each window) or the weights of a label (a scale for
+ * each label).  A row without a magnitude of 2^-119 or more: q = 0, scale 0.  A row that holds NaN or infinity: q = 0, scale NaN.
+ */
+int apr_quantize_rows_device(apr_engine *e, int dtype, const void *d_x, size_t n, size_t k, size_t ld, int8_t *d_q, size_t ld_q,
+                             float *d_scale);
+
+/*
+ * out[i][j] = (sum_k x[i][k] * w[j][k]) * x_scale[i] * w_scale[j] + bias[j]: x [m][k], w [n][k] (the weight of torch.nn.Linear),
+ * d_bias may be NULL.  The sum is exact (32-bit whole numbers), the rest is f32, rounded once to `dtype` (beyond its range:
+ * infinity).  1 <= k <= APR_LINEAR_MAX_K; m, n <= APR_LINEAR_MAX_ROWS.  Any alignment and stride; x and w that are 16-byte
+ * aligned with strides of a multiple of 16 are read 16 bytes at a time.
+ */
+int apr_linear_i8_device(apr_engine *e, const int8_t *d_x, size_t ld_x, const float *d_x_scale, const int8_t *d_w, size_t ld_w,
+                         const float *d_w_scale, const float *d_bias, size_t m, size_t n, size_t k, int dtype, void *d_out,
+                         size_t ld_out);
 
 /* Block until all work queued on this engine's stream has finished. */
 int apr_sync(apr_engine *e);

@@ -4,6 +4,7 @@
 // which is how the matrix instruction wants them: a lane holds 16 consecutive k of one row.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "element.hip.h"
@@ -21,42 +22,312 @@ struct LinearI8Args {
     unsigned m, n, k;
 };
 
-// 64 x 64 outputs at a time, four waves of 32 x 32; 64 k a step through LDS, byte by byte: any alignment.
-template <typename T>
-__global__ __launch_bounds__(256) void linear_i8_kernel(LinearI8Args a)
+// ---- tiled kernel: operands 16 bytes at a time, straight from memory to LDS ----
+//
+// A stage is BK bytes of k of every row of the tile, [row][BK / 16 units of 16 bytes]; unit c of row r lies at place
+// c ^ swizzle(r), so that the eight lanes that an LDS read serves together hit all banks once (rows are 64 or 128 bytes, which
+// alone would put the same unit of all rows on the same banks).  A DMA instruction fills 1 KiB of LDS lane by lane; the swizzle
+// is which unit each lane asks for.  Rows past the matrix and units past k are out of the buffer's range, which reads as 0.
+// LDS-DMA: 64 lanes x 16 B from a buffer to 1 KiB of LDS at byte address lds (wave-uniform).  The caller waits on vmcnt.
+__device__ __forceinline__ void linear_dma(i32x4 rs, unsigned voff, unsigned lds)
 {
-    __shared__ __align__(16) int8_t s_x[64][80], s_w[64][80];   // 80: neighbouring rows start in other banks
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    const unsigned long long tiles_n = (a.n + 63u) / 64u, tiles = (a.m + 63u) / 64u * tiles_n;
-    for (unsigned long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const unsigned m0 = (unsigned)(tile / tiles_n) * 64u, n0 = (unsigned)(tile % tiles_n) * 64u;
-        i32x16 acc = {};
-        for (unsigned k0 = 0; k0 < a.k; k0 += 64) {
-            __syncthreads();
-            for (unsigned i = threadIdx.x; i < 64 * 64; i += 256) {
-                const unsigned r = i >> 6, c = i & 63, k = k0 + c;
-                s_x[r][c] = m0 + r < a.m && k < a.k ? a.x[(m0 + r) * a.ld_x + k] : (int8_t)0;
-                s_w[r][c] = n0 + r < a.n && k < a.k ? a.w[(n0 + r) * a.ld_w + k] : (int8_t)0;
-            }
-            __syncthreads();
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(rs), "s"(lds)
+                 : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_dma_and_meet()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// the 256 or so tiles that run together share rows of x and w in their XCD's L2: the tiles are cut into one run for each of the
+// 8 XCDs (workgroups go to them in turn), and a run walks G tiles down m for each step along n
+__device__ __forceinline__ void linear_tile(unsigned block, unsigned tiles_m, unsigned tiles_n, unsigned &tm, unsigned &tn)
+{
+    const unsigned tiles = tiles_m * tiles_n, xcd = block & 7u, q = tiles >> 3, r = tiles & 7u;
+    const unsigned t = xcd * q + min(xcd, r) + (block >> 3);
+    const unsigned G = 8, per = G * tiles_n, g = t / per, in = t - g * per;
+    const unsigned rows = min(G, tiles_m - g * G);
+    tn = in / rows;
+    tm = g * G + in - tn * rows;
+}
+
+template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI8Args a, unsigned tiles_m, unsigned tiles_n)
+{
+    constexpr int WAVES = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32, KS = BK / 32, UNITS = BK / 16, RPD = 64 / UNITS;
+    constexpr int DA = BM / RPD / WAVES, DB = BN / RPD / WAVES, ABYTES = BM * BK, STAGE = (BM + BN) * BK;
+    extern __shared__ __align__(128) int8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned tm, tn;
+    linear_tile(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    tm = __builtin_amdgcn_readfirstlane(tm);   // the division is vector code
+    tn = __builtin_amdgcn_readfirstlane(tn);
+    const unsigned m0 = tm * BM, n0 = tn * BN;
+    const unsigned rows_x = min((unsigned)BM, a.m - m0), rows_w = min((unsigned)BN, a.n - n0);
+    const unsigned k16 = (a.k + 15u) & ~15u;
+    const unsigned ld_x = (unsigned)a.ld_x, ld_w = (unsigned)a.ld_w;
+    unsigned long long bx = (unsigned long long)(a.x + (unsigned long long)m0 * a.ld_x), bw = (unsigned long long)(a.w + (unsigned long long)n0 * a.ld_w);
+    // Range of the tile's rows: a row past the matrix begins beyond it (k16 <= ld) and reads as 0, at every stage, since a stage moves
+    // the base along k and not the range
+    const unsigned nx = (rows_x - 1) * ld_x + k16, nw = (rows_w - 1) * ld_w + k16;
+
+    // this lane's row and unit of a DMA instruction
+    const int dr = lane / UNITS, dp = lane % UNITS;
+    constexpr int SH = UNITS == 8 ? 0 : 1;
+    unsigned vx[DA], vw[DB];
+    const int du = dp ^ ((dr >> SH) & (UNITS - 1));   // RPD is a multiple of the swizzle's period
 #pragma unroll
-            for (int kk = 0; kk < 64; kk += 32) {
-                const i32x4 xa = *(const i32x4 *)&s_x[wm + (lane & 31)][kk + 16 * (lane >> 5)];
-                const i32x4 wb = *(const i32x4 *)&s_w[wn + (lane & 31)][kk + 16 * (lane >> 5)];
-                acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(xa, wb, acc, 0, 0, 0);
-            }
+    for (int i = 0; i < DA; i++) vx[i] = (unsigned)((wave * DA + i) * RPD + dr) * ld_x + 16u * du;
+#pragma unroll
+    for (int i = 0; i < DB; i++) vw[i] = (unsigned)((wave * DB + i) * RPD + dr) * ld_w + 16u * du;
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) int8_t *)lds;
+
+    const unsigned full = a.k / BK, steps = (a.k + BK - 1) / BK;
+    unsigned k_next = 0;   // first k of the next stage to fetch
+    int slot_in = 0;
+    auto fetch = [&]() {
+        if (k_next < a.k) {
+            const i32x4 rx = {(int)(unsigned)bx, (int)(unsigned)(bx >> 32), (int)nx, 0x00020000};
+            const i32x4 rw = {(int)(unsigned)bw, (int)(unsigned)(bw >> 32), (int)nw, 0x00020000};
+            const bool tail = k_next + BK > a.k;
+            const bool out = tail && k_next + 16u * du >= a.k;
+            const unsigned base = lds0 + slot_in * STAGE + wave * DA * 1024, basew = lds0 + slot_in * STAGE + ABYTES + wave * DB * 1024;
+#pragma unroll
+            for (int i = 0; i < DA; i++) linear_dma(rx, out ? 0xFFFFFFF0u : vx[i], base + i * 1024);
+#pragma unroll
+            for (int i = 0; i < DB; i++) linear_dma(rw, out ? 0xFFFFFFF0u : vw[i], basew + i * 1024);
+            bx += BK; bw += BK;
+        } else {
+            // an empty stage keeps the count of loads in flight: all lanes out of range
+            const i32x4 r0 = {(int)(unsigned)(unsigned long long)a.x, (int)(unsigned)((unsigned long long)a.x >> 32), 0, 0x00020000};
+            const unsigned base = lds0 + slot_in * STAGE + wave * DA * 1024, basew = lds0 + slot_in * STAGE + ABYTES + wave * DB * 1024;
+#pragma unroll
+            for (int i = 0; i < DA; i++) linear_dma(r0, 0xFFFFFFF0u, base + i * 1024);
+#pragma unroll
+            for (int i = 0; i < DB; i++) linear_dma(r0, 0xFFFFFFF0u, basew + i * 1024);
         }
-        const unsigned n = n0 + wn + (lane & 31);
-        if (n < a.n) {
-            const float ws = a.w_scale[n], b = a.bias ? a.bias[n] : 0.0f;
+        k_next += BK;
+        slot_in = slot_in + 1 == NBUF ? 0 : slot_in + 1;
+    };
+
+    const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN), r32 = lane & 31, half = lane >> 5;
+    unsigned pa[KS];   // this lane's place in a row for each k of 32
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const unsigned m = m0 + wm + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-                if (m < a.m) ((T *)a.out)[m * a.ld_out + n] = from_f32<T>((float)acc[i] * a.x_scale[m] * ws + b);
+    for (int kk = 0; kk < KS; kk++) pa[kk] = (unsigned)(((2 * kk + half) ^ ((r32 >> SH) & (UNITS - 1))) * 16);
+    const int8_t *la = lds + (wm + r32) * BK, *lb = lds + ABYTES + (wn + r32) * BK;
+
+    i32x16 acc[FM][FN] = {};
+    i32x4 fa[2][FM], fb[2][FN];
+    auto read = [&](int set, unsigned stage, int kk) {
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[set][i] = *(const i32x4 *)(la + stage + i * 32 * BK + pa[kk]);
+#pragma unroll
+        for (int j = 0; j < FN; j++) fb[set][j] = *(const i32x4 *)(lb + stage + j * 32 * BK + pa[kk]);
+    };
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[set][j], fa[set][i], acc[i][j], 0, 0, 0);
+    };
+
+    constexpr int FLY = (NBUF - 2) * (DA + DB);   // loads that may still be on their way when the next stage has to be there
+#pragma unroll
+    for (int s = 0; s < NBUF - 1; s++) fetch();
+    wait_dma_and_meet<FLY>();
+    unsigned stage = 0;
+    if (full) read(0, 0, 0);
+    for (unsigned s = 0; s < full; s++) {
+        fetch();   // into the stage that was read before the last meeting
+        const unsigned next = stage + STAGE == NBUF * STAGE ? 0 : stage + STAGE;
+#pragma unroll
+        for (int kk = 0; kk < KS; kk++) {
+            if (kk + 1 < KS) read((kk + 1) & 1, stage, kk + 1);
+            else {
+                wait_dma_and_meet<FLY>();
+                read(0, next, 0);   // past the last whole stage: the tail's, or zeros
             }
+            multiply(kk & 1);
+        }
+        stage = next;
+    }
+    if (steps > full) {
+        // the tail: units past k are 0; the unit that k ends in is cut in x, which is enough
+#pragma unroll
+        for (int kk = 0; kk < KS; kk++) {
+            read(kk & 1, stage, kk);
+            const int left = (int)a.k - (int)(full * BK + 32 * kk + 16 * half);
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const int keep = left - 4 * d;
+                const int mask = keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+#pragma unroll
+                for (int i = 0; i < FM; i++) fa[kk & 1][i][d] &= mask;
+            }
+            multiply(kk & 1);
         }
     }
+    // The end of a tile.  w is the instruction's first operand, so a lane holds runs of four neighbouring n of one m: 32 rows of the
+    // wave's outputs at a time go through the wave's own piece of the LDS and out again in whole 16-byte units of a row.
+    constexpr int TN = BN / WN, ROW = TN * (int)sizeof(T) + 16;   // + 16: rows start in other banks
+    static_assert(WAVES * 32 * ROW + 2 * BN * 4 <= NBUF * STAGE, "the outputs fit in the stages");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // every stage is read, every load has landed
+    float *s_ws = (float *)(lds + WAVES * 32 * ROW), *s_b = s_ws + BN;
+    for (int c = threadIdx.x; c < BN; c += WAVES * 64) {
+        const bool in = n0 + c < a.n;
+        s_ws[c] = in ? a.w_scale[n0 + c] : 0.0f;
+        s_b[c] = in && a.bias ? a.bias[n0 + c] : 0.0f;
+    }
+    __syncthreads();
+    int8_t *mine = lds + wave * 32 * ROW;
+    constexpr int V = 16 / (int)sizeof(T), LPR = TN / V, RPI = 64 / LPR;   // values of a unit, lanes a row, rows an instruction
+    typedef T tx4 __attribute__((ext_vector_type(4)));
+    typedef T txv __attribute__((ext_vector_type(V)));
+    const bool units = ((a.ld_out * sizeof(T) | (unsigned long long)a.out) & 15) == 0;
+    T *out = (T *)a.out + (unsigned long long)m0 * a.ld_out + n0 + wn;
+    const unsigned m_left = a.m - m0, n_left = a.n - n0 > (unsigned)wn ? a.n - n0 - wn : 0;
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const unsigned mr = wm + 32 * i;
+        const float xs = mr + r32 < m_left ? a.x_scale[m0 + mr + r32] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int c = 32 * j + 8 * g + 4 * half;
+                tx4 v;
+#pragma unroll
+                for (int q = 0; q < 4; q++) v[q] = from_f32<T>((float)acc[i][j][4 * g + q] * xs * s_ws[wn + c + q] + s_b[wn + c + q]);
+                *(tx4 *)(mine + r32 * ROW + c * (int)sizeof(T)) = v;
+            }
+        __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
+        if (units) {
+#pragma unroll
+            for (int r = 0; r < 32; r += RPI) {
+                const unsigned row = r + lane / LPR, c = lane % LPR * V;
+                const txv v = *(const txv *)(mine + row * ROW + c * sizeof(T));
+                T *o = out + (mr + row) * a.ld_out + c;
+                if (mr + row < m_left) {
+                    if (c + V <= n_left) *(txv *)o = v;
+                    else
+                        for (int q = 0; q < V; q++)
+                            if (c + q < n_left) o[q] = v[q];
+                }
+            }
+        } else {
+#pragma unroll 8
+            for (int r = 0; r < TN / 2; r++) {
+                const unsigned idx = 64 * r + lane, row = idx / TN, c = idx % TN;
+                if (mr + row < m_left && c < n_left) out[(mr + row) * a.ld_out + c] = *(const T *)(mine + row * ROW + c * sizeof(T));
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- few tiles: every wave takes a part of k for the same 32 x 32 outputs, straight from memory to registers ----
+//
+// Blocks of 128 k go to the W waves in turn; a lane reads the four 16-byte units of its row that the block's four matrix instructions
+// want (they share the row's cache lines).  The waves' partial sums, exact whole numbers, meet in LDS.
+// WHOLE: the rows are 16-byte aligned, and the unit that k ends in is read whole (it lies in the row's stride) and cut in x.
+// Otherwise a unit begins at any byte, and the one that k ends in is read byte by byte.
+template <bool WHOLE>
+__device__ __forceinline__ i32x4 linear_unit(const int8_t *row, unsigned k, unsigned end)
+{
+    i32x4 v = {0, 0, 0, 0};
+    if (k >= end) return v;
+    if (WHOLE) return *(const i32x4 *)(row + k);
+    if (k + 16u <= end) {
+        __builtin_memcpy(&v, row + k, 16);
+        return v;
+    }
+    for (unsigned c = 0; k + c < end; c++) v[c >> 2] |= (int)(uint8_t)row[k + c] << (8 * (c & 3));
+    return v;
+}
+
+template <typename T, int W, bool WHOLE>
+__global__ __launch_bounds__(W * 64, 1) void linear_i8_few_kernel(LinearI8Args a)
+{
+    __shared__ int s_part[W][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+    const unsigned long long tiles_n = (a.n + 31u) / 32u, tiles = (a.m + 31u) / 32u * tiles_n;
+    const unsigned blocks = (a.k + 127u) / 128u;
+    for (unsigned long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const unsigned m0 = (unsigned)(tile / tiles_n) * 32u, n0 = (unsigned)(tile % tiles_n) * 32u;
+        const unsigned k_x = m0 + r32 < a.m ? a.k : 0, k_w = n0 + r32 < a.n ? a.k : 0;   // a row past the matrix has no units
+        const int8_t *x = a.x + (m0 + r32) * a.ld_x, *w = a.w + (n0 + r32) * a.ld_w;
+        i32x16 acc = {};
+        i32x4 fx[4], fw[4];
+        auto load = [&](unsigned b) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                fw[u] = linear_unit<WHOLE>(w, b * 128u + 32u * u + 16u * half, k_w);
+                fx[u] = linear_unit<WHOLE>(x, b * 128u + 32u * u + 16u * half, k_x);
+            }
+        };
+        load(wave);
+        for (unsigned b = wave; b < blocks; b += W) {
+            if (WHOLE && b * 128u + 128u > a.k) {
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        const int keep = (int)a.k - (int)(b * 128u + 32u * u + 16u * half) - 4 * d;
+                        fx[u][d] &= keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[u], fw[u], acc, 0, 0, 0);
+            load(b + W);
+        }
+        __syncthreads();   // the last tile's sums are read
+#pragma unroll
+        for (int e = 0; e < 16; e++) s_part[wave][e][lane] = acc[e];
+        __syncthreads();
+        for (int e = wave; e < 16; e += W) {
+            int sum = 0;
+#pragma unroll
+            for (int v = 0; v < W; v++) sum += s_part[v][e][lane];
+            const unsigned m = m0 + 8 * (e >> 2) + 4 * half + (e & 3), n = n0 + r32;
+            if (m < a.m && n < a.n) ((T *)a.out)[m * a.ld_out + n] = from_f32<T>((float)sum * a.x_scale[m] * a.w_scale[n] + (a.bias ? a.bias[n] : 0.0f));
+        }
+    }
+}
+
+// ---- which kernel ----
+//
+// Microseconds of a variant: t0 for each tile that a CU walks one after the other, and a step of 128 k takes `alone` (its latency,
+// shared by the `beside` tiles that fit a CU together) or `full` for each tile (its throughput), whichever is longer.  Measured with
+// one to eight rounds of tiles, bf16 out; 1024 x 8192 x 8192: 98 / 73 / 121 / 103 us by 256 x 256, 128 x 128, 64 x 64 with four and with
+// two stages (the rule: 98 / 73 / 126 / 108), 256 x 8192 x 8192: 85 / 50 / 32 / 39 (98 / 50 / 32 / 39), 16384 x 8192 x 8192: 925 / 1113 / 1780 / 1612.
+// The `few` kernel: per 32 x 32 tile of a CU 2.5 us and 1.9 us for each 1024 k: 256 x 527 x 1024 takes 4.4 us against 6.7, 4096 x 527 x 1024 30 against 9.4.
+struct LinearCost {
+    int tile, beside;
+    float t0, alone, full;
+};
+constexpr LinearCost kLinearCost[4] = {{256, 1, 5.0f, 1.45f, 1.72f}, {128, 2, 3.6f, 0.73f, 0.54f}, {64, 2, 2.5f, 0.30f, 0.24f}, {64, 5, 2.5f, 0.57f, 0.20f}};
+enum { kLinear256, kLinear128, kLinear64Deep, kLinear64, kLinearFew };
+
+inline int linear_variant(unsigned m, unsigned n, unsigned k, int n_cus)
+{
+    const float steps = (float)((k + 127) / 128), cus = (float)n_cus;
+    const float few_tiles = (float)((m + 31) / 32) * (float)((n + 31) / 32);
+    float best = ceilf(few_tiles / cus) * (2.5f + 1.9e-3f * (float)k);
+    int variant = kLinearFew;
+    for (int v = 0; v < 4; v++) {
+        const LinearCost &c = kLinearCost[v];
+        const float tiles = (float)((m + c.tile - 1) / c.tile) * (float)((n + c.tile - 1) / c.tile);
+        const float per_cu = ceilf(tiles / cus), rounds = ceilf(per_cu / (float)c.beside);
+        const float us = c.t0 * rounds + steps * fmaxf(c.alone * rounds, c.full * per_cu);
+        if (us < best) { best = us; variant = v; }
+    }
+    return variant;
 }
 
 }  // namespace apr

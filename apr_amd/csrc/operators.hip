@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <type_traits>
@@ -61,6 +62,39 @@ void with_type(int dtype, F f)
     else f((bf16_t *)nullptr);
 }
 #define APR_TYPE_OF(p) std::remove_pointer_t<decltype(p)>
+
+// Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.
+template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN>
+void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
+{
+    constexpr int bytes = (BM + BN) * BK * NBUF;
+    const auto kernel = linear_i8_tile_kernel<T, BM, BN, BK, NBUF, WM, WN>;
+    static std::atomic<uint64_t> allowed{0};
+    const uint64_t bit = 1ull << (v.device & 63);
+    if (bytes > 65536 && !(allowed.load(std::memory_order_relaxed) & bit)) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
+    const unsigned tiles_m = (a.m + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN;
+    hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n), dim3(WM * WN * 64), bytes, v.stream, a, tiles_m, tiles_n);
+}
+
+template <typename T>
+void launch_linear(const EngineView &v, const LinearI8Args &a)
+{
+    const unsigned long long few = (unsigned long long)((a.m + 31) / 32) * ((a.n + 31) / 32);
+    const dim3 few_grid((unsigned)std::min<unsigned long long>(few, kMostBlocks));
+    const bool whole = aligned(a.x, 16) && aligned(a.w, 16) && a.ld_x % 16 == 0 && a.ld_w % 16 == 0;
+    int variant = linear_variant(a.m, a.n, a.k, v.n_cus);
+    // the tiles address their rows with 32 bits, and a grid has less than 2^32 threads
+    if (a.ld_x > (1u << 22) || a.ld_w > (1u << 22) || few > (1ull << 24)) variant = kLinearFew;
+    if (!whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 4, false>), few_grid, dim3(256), 0, v.stream, a);
+    else if (variant == kLinearFew) hipLaunchKernelGGL((linear_i8_few_kernel<T, 16, true>), few_grid, dim3(1024), 0, v.stream, a);
+    else if (variant == kLinear256) launch_linear_tiles<T, 256, 256, 128, 2, 2, 4>(v, a);
+    else if (variant == kLinear128) launch_linear_tiles<T, 128, 128, 128, 2, 2, 2>(v, a);
+    else if (variant == kLinear64Deep) launch_linear_tiles<T, 64, 64, 128, 4, 2, 2>(v, a);
+    else launch_linear_tiles<T, 64, 64, 128, 2, 2, 2>(v, a);
+}
 
 }  // namespace
 
@@ -163,11 +197,8 @@ int apr_linear_i8_device(apr_engine *e, const int8_t *d_x, size_t ld_x, const fl
     LinearI8Args a;
     a.x = d_x; a.w = d_w; a.x_scale = d_x_scale; a.w_scale = d_w_scale; a.bias = d_bias; a.out = d_out;
     a.ld_x = ld_x; a.ld_w = ld_w; a.ld_out = ld_out; a.m = (unsigned)m; a.n = (unsigned)n; a.k = (unsigned)k;
-    const unsigned long long tiles = ((m + 63) / 64) * ((n + 63) / 64);
     return on_engine(e, me, [&](const EngineView &v) {
-        with_type(dtype, [&](auto *p) {
-            hipLaunchKernelGGL(linear_i8_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<unsigned long long>(tiles, kMostBlocks)), dim3(256), 0, v.stream, a);
-        });
+        with_type(dtype, [&](auto *p) { launch_linear<APR_TYPE_OF(p)>(v, a); });
     });
 }
 

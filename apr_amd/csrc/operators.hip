@@ -63,6 +63,25 @@ void with_type(int dtype, F f)
 }
 #define APR_TYPE_OF(p) std::remove_pointer_t<decltype(p)>
 
+template <typename T>
+void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPlan &p)
+{
+    if (!p.threads) {
+        const dim3 grid((unsigned)std::min<unsigned long long>((a.n + 3) / 4, kMostBlocks)), block(256);
+        if (p.each == 1) hipLaunchKernelGGL((logprob_wave_kernel<T, 1>), grid, block, 0, v.stream, a);
+        else if (p.each == 2) hipLaunchKernelGGL((logprob_wave_kernel<T, 2>), grid, block, 0, v.stream, a);
+        else if (p.each == 4) hipLaunchKernelGGL((logprob_wave_kernel<T, 4>), grid, block, 0, v.stream, a);
+        else if (p.each == 8) hipLaunchKernelGGL((logprob_wave_kernel<T, 8>), grid, block, 0, v.stream, a);
+        else hipLaunchKernelGGL((logprob_wave_kernel<T, 16>), grid, block, 0, v.stream, a);
+        return;
+    }
+    const dim3 grid((unsigned)std::min<unsigned long long>(a.n * a.pieces, kMostBlocks));
+    if (p.threads == 1024) hipLaunchKernelGGL((logprob_block_kernel<T, 1024, 32>), grid, dim3(1024), 0, v.stream, a);
+    else if (p.threads == 512) hipLaunchKernelGGL((logprob_block_kernel<T, 512, 32>), grid, dim3(512), 0, v.stream, a);
+    else if (p.each == 32) hipLaunchKernelGGL((logprob_block_kernel<T, 256, 32>), grid, dim3(256), 0, v.stream, a);
+    else hipLaunchKernelGGL((logprob_block_kernel<T, 256, 16>), grid, dim3(256), 0, v.stream, a);
+}
+
 // Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.
 template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN>
 void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
@@ -102,8 +121,8 @@ extern "C" {
 
 size_t apr_label_logprobs_workspace(size_t n, size_t n_labels, int top)
 {
-    (void)n; (void)n_labels; (void)top;
-    return 0;
+    if (n < 1 || n > kMostRows || n_labels < 1 || n_labels > kMostRows || top < 0 || top > APR_MAX_TOP) return 0;
+    return logprob_plan(n, n_labels, top).work;
 }
 
 int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld, double scale,
@@ -129,10 +148,13 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
     LogprobArgs a;
     a.x = d_logits; a.n = n; a.ld = ld; a.n_labels = (unsigned)n_labels; a.scale = (float)scale; a.target = d_target; a.top = top;
     a.logprob = d_logprob; a.entropy = d_entropy; a.stat = d_stat; a.top_label = d_top_label; a.top_logprob = d_top_logprob;
+    const LogprobPlan plan = logprob_plan(n, n_labels, top);
+    a.pieces = plan.pieces; a.piece_len = plan.piece_len;
+    a.part_top = (unsigned long long *)d_work;
+    a.part = (LogprobPart *)((char *)d_work + (plan.pieces > 1 ? n * plan.pieces * (size_t)top * 8 : 0));
     return on_engine(e, me, [&](const EngineView &v) {
-        with_type(dtype, [&](auto *p) {
-            hipLaunchKernelGGL(logprob_rows_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(256), 0, v.stream, a);
-        });
+        with_type(dtype, [&](auto *p) { launch_logprobs<APR_TYPE_OF(p)>(v, a, plan); });
+        if (plan.pieces > 1) hipLaunchKernelGGL(logprob_join_kernel, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(64), 0, v.stream, a, dtype);
     });
 }
 

@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "element.hip.h"
 
 namespace apr {
@@ -102,11 +104,13 @@ struct ExpSum {
     }
 };
 
-// The outputs of a row from its sums; called by one lane.
-__device__ __forceinline__ void logprob_write(const LogprobArgs &a, unsigned long long row, LogprobPart r, float x_target, bool has_target)
+// log of a sum of exponentials: 1 <= s, or 0, or NaN; the instruction's error is 2^-24 of log2 s or of 1
+__device__ __forceinline__ float log_of_sum(float s) { return __builtin_amdgcn_logf(s) * 0.69314718055994530942f; }
+
+// The outputs of a row from its sums and their logarithm; called by one lane.
+__device__ __forceinline__ void logprob_write(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, float x_target, bool has_target)
 {
     const bool bad = r.s != r.s, empty = r.m == kNegInf && !bad;
-    const float log_s = logf(r.s);
     if (a.stat) {
         a.stat[2 * row] = bad ? kNaN : r.m;
         a.stat[2 * row + 1] = bad ? kNaN : log_s;
@@ -114,11 +118,11 @@ __device__ __forceinline__ void logprob_write(const LogprobArgs &a, unsigned lon
     if (a.entropy) a.entropy[row] = bad ? kNaN : empty ? 0.0f : fmaxf(log_s - a.scale * (r.u / r.s), 0.0f);
     if (a.logprob) a.logprob[row] = !has_target ? 0.0f : bad ? kNaN : empty ? kNegInf : a.scale * (x_target - r.m) - log_s;
 }
-__device__ __forceinline__ void logprob_write_top(const LogprobArgs &a, unsigned long long row, LogprobPart r, int place, unsigned long long key)
+__device__ __forceinline__ void logprob_write_top(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, int place, unsigned long long key)
 {
     const bool bad = r.s != r.s, none = bad || !key;
     if (a.top_label) a.top_label[row * a.top + place] = none ? -1 : key_label(key);
-    if (a.top_logprob) a.top_logprob[row * a.top + place] = bad ? kNaN : none ? kNegInf : a.scale * (key_score(key) - r.m) - logf(r.s);
+    if (a.top_logprob) a.top_logprob[row * a.top + place] = bad ? kNaN : none ? kNegInf : a.scale * (key_score(key) - r.m) - log_s;
 }
 
 // ---- the best `top` of many keys, by one wave ----
@@ -139,18 +143,6 @@ __device__ __forceinline__ float reached_by(float v, int top)
     return key_score((unsigned long long)t << 32);
 }
 
-// The `top`-th largest of the keys that count() counts (each key is there once): the largest K that at least `top` of them reach.
-template <typename F>
-__device__ __forceinline__ unsigned long long key_reached_by(int top, F count)
-{
-    unsigned long long t = 0;
-    for (int b = 63; b >= 0; b--) {
-        const unsigned long long c = t | (1ull << b);
-        if (count(c) >= top) t = c;
-    }
-    return t;
-}
-
 // Place of a lane's key among the first n lanes' keys, best first
 __device__ __forceinline__ int key_place(unsigned long long key, int n)
 {
@@ -163,28 +155,87 @@ __device__ __forceinline__ int key_place(unsigned long long key, int n)
     return place;
 }
 
-// Keeps the best `top` of the n keys in `list` (LDS, n <= 16 * 64) there, in any order; returns how many that are (<= 64)
-__device__ __forceinline__ int keep_best(unsigned long long *list, int n, int top, int lane)
+// Of the wave's keys k[0..N-1] (0: none) at most 64 that hold the best `top` are left in `list` (LDS); returns how many, and in
+// `border` a key that none of the dropped ones reaches.  Counting reached candidates of a binary search: 16 bits of the score first, and
+// if equal scores leave more than 64, all other bits, which ends at the `top`-th key itself, as every key is there once.
+template <int N>
+__device__ __forceinline__ int keep_best(const unsigned long long (&k)[N], int top, int lane, unsigned long long *list, unsigned long long &border)
 {
-    if (n <= 64) return n;
-    unsigned long long k[16];
+    uint32_t t = 0;
 #pragma unroll
-    for (int i = 0; i < 16; i++) k[i] = 64 * i + lane < n ? list[64 * i + lane] : 0;
-    const unsigned long long t = key_reached_by(top, [&](unsigned long long c) {
+    for (int b = 31; b >= 16; b--) {
+        const uint32_t c = t | (1u << b);
         int count = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) count += __builtin_popcountll(__ballot(k[i] >= c));
-        return count;
-    });
-    int kept = 0;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const unsigned long long in = __ballot(k[i] >= t && k[i]);
-        if (k[i] >= t && k[i]) list[kept + __builtin_popcountll(in & ((1ull << lane) - 1))] = k[i];
-        kept += __builtin_popcountll(in);
+        for (int i = 0; i < N; i++) count += __builtin_popcountll(__ballot((uint32_t)(k[i] >> 32) >= c));
+        if (count >= top) t = c;
     }
-    return kept;
+    unsigned long long reach = (unsigned long long)t << 32;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) n += __builtin_popcountll(__ballot(k[i] >= reach && k[i]));
+    if (n > 64)
+        for (int b = 47; b >= 0; b--) {
+            const unsigned long long c = reach | (1ull << b);
+            int count = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) count += __builtin_popcountll(__ballot(k[i] >= c));
+            if (count >= top) reach = c;
+        }
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const bool in = k[i] >= reach && k[i];
+        const unsigned long long mask = __ballot(in);
+        if (in) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = k[i];
+        n += __builtin_popcountll(mask);
+    }
+    border = reach;
+    return n;
 }
+
+// The alternatives of a row from at most 64 keys in `list`
+__device__ __forceinline__ void logprob_write_list(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, const unsigned long long *list, int n, int lane)
+{
+    const unsigned long long key = lane < n ? list[lane] : 0;
+    const int place = key_place(key, n);
+    if (lane < n && place < a.top) logprob_write_top(a, row, r, log_s, place, key);
+    if (lane >= n && lane < a.top) logprob_write_top(a, row, r, log_s, lane, 0);
+}
+
+// A wave's candidates for the alternatives, collected in LDS as its scores come by, 64 lanes at a time.  Taken are scores of at least
+// `least` whose key passes `border`; when the list is full, the best are kept and both rise.
+constexpr int kList = 128;
+struct Candidates {
+    unsigned long long *list, border = 0;
+    int n = 0;
+    float least = __builtin_inff();
+    __device__ __forceinline__ explicit Candidates(unsigned long long *l) : list(l) {}
+    __device__ __forceinline__ void shrink(int top, int lane)
+    {
+        __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
+        unsigned long long k[kList / 64];
+#pragma unroll
+        for (int i = 0; i < kList / 64; i++) k[i] = 64 * i + lane < n ? list[64 * i + lane] : 0;
+        __builtin_amdgcn_wave_barrier();
+        n = keep_best(k, top, lane, list, border);
+        least = fmaxf(least, key_score(border));
+        __builtin_amdgcn_wave_barrier();
+    }
+    // one score of every lane
+    __device__ __forceinline__ void offer(float v, unsigned label, int top, int lane)
+    {
+        if (!__ballot(v >= least)) return;
+        const unsigned long long key = score_key(v, label);
+        unsigned long long mask = __ballot(v >= least && key >= border);
+        if (n + __builtin_popcountll(mask) > kList) {   // then n > 64, and no more than 64 are left
+            shrink(top, lane);
+            mask = __ballot(v >= least && key >= border);
+        }
+        if (mask >> lane & 1) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = key;
+        n += __builtin_popcountll(mask);
+    }
+};
 
 // ---- short rows: a wave per row, E scores a lane ----
 //
@@ -192,9 +243,8 @@ __device__ __forceinline__ int keep_best(unsigned long long *list, int n, int to
 template <typename T, int E>
 __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
 {
-    __shared__ unsigned long long s_list[4][64];
+    __shared__ unsigned long long s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned long long *list = s_list[wave];
     for (unsigned long long row = (unsigned long long)blockIdx.x * 4 + wave; row < a.n; row += (unsigned long long)gridDim.x * 4) {
         const T *x = (const T *)a.x + row * a.ld;
         const int t = a.target ? a.target[row] : -1;
@@ -202,7 +252,7 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         const float xt = has_t ? to_f32(x[t]) : 0.0f;
         float v[E], best = kNegInf;
 #pragma unroll
-        for (int i = 0; i < E; i++) v[i] = 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf;
+        for (int i = 0; i < E; i++) v[i] = i < E - 1 || 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf;
 #pragma unroll
         for (int i = 0; i < E; i++) best = fmaxf(best, v[i]);
         LogprobPart r;
@@ -212,174 +262,149 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         for (int i = 0; i < E; i++) sum.add(v[i]);
         r.s = wave_reduce(sum.s, SumOf());
         r.u = wave_reduce(sum.u, SumOf());
-        if (lane == 0) logprob_write(a, row, r, xt, has_t);
+        const float log_s = log_of_sum(r.s);
+        if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
-        const float least = reached_by(best, a.top);
-        int n = 0;
+        Candidates c(s_list[wave]);
+        c.least = reached_by(best, a.top);
 #pragma unroll
-        for (int i = 0; i < E; i++) n += __builtin_popcountll(__ballot(v[i] >= least));
-        unsigned long long reach = 0;
-        if (n > 64)   // many equal scores: the exact border, over the scores in memory (this is rare, and they would take registers)
-            reach = key_reached_by(a.top, [&](unsigned long long c) {
-                int count = 0;   // lane 0 is in every round
-                for (unsigned j = lane; j < a.n_labels; j += 64) {
-                    const float y = to_f32(x[j]);
-                    count += __builtin_popcountll(__ballot(y >= least && score_key(y, j) >= c));
-                }
-                return __builtin_amdgcn_readfirstlane(count);
-            });
-        n = 0;
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const unsigned long long key = score_key(v[i], 64 * i + lane);
-            const bool in = v[i] >= least && key >= reach;
-            const unsigned long long mask = __ballot(in);
-            if (in) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = key;
-            n += __builtin_popcountll(mask);
-        }
-        __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
-        const unsigned long long key = lane < n ? list[lane] : 0;
-        const int place = key_place(key, n);
-        if (lane < n && place < a.top) logprob_write_top(a, row, r, place, key);
-        if (lane >= n && lane < a.top) logprob_write_top(a, row, r, lane, 0);
+        for (int i = 0; i < E; i++) c.offer(v[i], 64 * i + lane, a.top, lane);
+        if (c.n > 64) c.shrink(a.top, lane);
+        __builtin_amdgcn_wave_barrier();
+        logprob_write_list(a, row, r, log_s, c.list, c.n, lane);
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-// ---- longer rows: a workgroup per row, or per piece of one; E scores a lane in registers, read once ----
+// ---- longer rows: a wave per row, or per piece of one, 1024 scores at a time, the next ones on their way ----
 //
+// No lane waits for another wave.  The sums are relative to a reference that the wave shares: the best score so far, renewed only
+// when a score passes it by more than kGap (then exp <= e^kGap, and nothing is lost: the sums are floating point), because the running
+// maximum itself would be new in some lane at nearly every step.  A step's 16 terms of a lane are summed before they are added.
 // 16-byte loads begin at the 16-byte unit that the piece begins in (which is inside the allocation, as the piece's first element is);
 // what does not belong to the piece counts as ruled out.
-// Candidates are the scores that at least `top` of 64 groups of NT / 64 lanes reach with their best; they are collected in LDS.
-// If equal scores make them too many, the exact border is found by counting over the whole workgroup.
-constexpr int kCandidates = 1024;
+constexpr float kGap = 8.0f;
 
-template <typename T, int NT, int E>
-__global__ __launch_bounds__(NT, 8) void logprob_block_kernel(LogprobArgs a)
+template <typename T>
+__global__ __launch_bounds__(256, 8) void logprob_stream_kernel(LogprobArgs a)
 {
-    constexpr int V = 16 / (int)sizeof(T), VECS = E / V, WAVES = NT / 64;
+    constexpr int V = 16 / (int)sizeof(T), U = 16 / V;
     typedef T txv __attribute__((ext_vector_type(V)));
-    __shared__ float s_group[64], s_s[WAVES], s_u[WAVES];
-    __shared__ unsigned long long s_list[kCandidates];
-    __shared__ int s_n;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ unsigned long long s_list[4][kList];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const unsigned long long works = a.n * a.pieces;
-    for (unsigned long long work = blockIdx.x; work < works; work += gridDim.x) {
+    const float c = a.scale * kLog2E, gap = kGap / a.scale, least_t = -200.0f / a.scale;
+    for (unsigned long long work = (unsigned long long)blockIdx.x * waves + wave; work < works; work += (unsigned long long)gridDim.x * waves) {
         const unsigned long long row = a.pieces == 1 ? work : work / a.pieces;
         const unsigned piece = (unsigned)(work - row * a.pieces), j0 = piece * a.piece_len, j1 = min(j0 + a.piece_len, a.n_labels);
         const T *x = (const T *)a.x + row * a.ld;
-        // first unit, and the label that its first element would be (modulo 2^32; below j0 by less than V)
         const unsigned off = (unsigned)(((unsigned long long)(x + j0) & 15) / sizeof(T));
         const txv *units = (const txv *)(x + j0 - off);
-        const unsigned len = j1 - j0 + off, n_units = (len + V - 1) / V;
-        float v[E], best = kNegInf;
+        const unsigned len = j1 - j0 + off, n_units = (len + V - 1) / V, steps = (n_units + 64 * U - 1) / (64 * U);
+        txv cur[U], next[U];
+        const auto load = [&](txv(&to)[U], unsigned step) {
 #pragma unroll
-        for (int q = 0; q < VECS; q++) {
-            const unsigned w = q * NT + threadIdx.x;
-            if (w < n_units) {
-                const txv p = units[w];
+            for (int q = 0; q < U; q++) {
+                const unsigned w = (step * U + q) * 64 + lane;
+                if (w < n_units) to[q] = units[w];
+                else to[q] = (T)kNegInf;
+            }
+        };
+        load(cur, 0);
+        float m = kNegInf, ref = kNegInf, s = 0.0f, u = 0.0f;
+        Candidates best(s_list[wave]);
+        for (unsigned step = 0; step < steps; step++) {
+            if (step + 1 < steps) load(next, step + 1);
+            float v[16], top = kNegInf;
 #pragma unroll
-                for (int i = 0; i < V; i++) v[q * V + i] = to_f32(p[i]);
-                if (w == 0 || w == n_units - 1) {
+            for (int e = 0; e < 16; e++) v[e] = to_f32(cur[e / V][e % V]);
+            if (step == 0 || step == steps - 1) {
 #pragma unroll
-                    for (int i = 0; i < V; i++)
-                        if (w * V + i < off || w * V + i >= len) v[q * V + i] = kNegInf;
+                for (int e = 0; e < 16; e++) {
+                    const unsigned at = ((step * U + e / V) * 64 + lane) * V + e % V;
+                    if (at < off || at >= len) v[e] = kNegInf;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) v[q * V + i] = kNegInf;
             }
-        }
-        const auto label = [&](int e) { return j0 - off + (e / V * NT + threadIdx.x) * V + e % V; };
 #pragma unroll
-        for (int e = 0; e < E; e++) best = fmaxf(best, v[e]);
-        const float group = NT == 1024 ? row_reduce(best, MaxOf()) : NT == 512 ? fmaxf(quad_reduce(best, MaxOf()), lane_move<0x141, 0xf>(quad_reduce(best, MaxOf())))
-                                                                                : quad_reduce(best, MaxOf());
-        if (threadIdx.x % (NT / 64) == 0) s_group[threadIdx.x / (NT / 64)] = group;
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
-        const float g = s_group[lane];
-        LogprobPart r;
-        r.m = wave_reduce(g, MaxOf());
-        ExpSum sum(r.m, a.scale);
+            for (int e = 0; e < 16; e++) top = fmaxf(top, v[e]);
+            m = fmaxf(m, top);
+            if (__ballot(top > ref + gap)) {
+                const float higher = fmaxf(wave_reduce(top, MaxOf()), ref), d = ref - higher, w = __builtin_amdgcn_exp2f(d * c);
+                u = w * fmaf(fmaxf(d, least_t), s, u);
+                s *= w;
+                ref = higher;
+            }
+            const float r = ref == kNegInf ? 0.0f : ref;
+            float es = 0.0f, eu = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; e++) sum.add(v[e]);
-        const float ws = wave_reduce(sum.s, SumOf()), wu = wave_reduce(sum.u, SumOf());
-        if (lane == 0) { s_s[wave] = ws; s_u[wave] = wu; }
-        if (a.top) {
-            const float least = reached_by(g, a.top);
-            if (best >= least) {
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (v[e] >= least) {
-                        const int at = atomicAdd(&s_n, 1);
-                        if (at < kCandidates) s_list[at] = score_key(v[e], label(e));
-                    }
+            for (int e = 0; e < 16; e++) {
+                const float t = v[e] - r, p = __builtin_amdgcn_exp2f(t * c);
+                es += p;
+                eu = fmaf(p, fmaxf(t, least_t), eu);
             }
-            __syncthreads();
-            if (s_n > kCandidates) {
-                // over the scores in memory: this is rare, and they would take registers
-                const unsigned long long reach = key_reached_by(a.top, [&](unsigned long long c) {
-                    int count = 0;   // lane 0 is in every round of its wave
-                    for (unsigned j = j0 + threadIdx.x; j < j1; j += NT) {
-                        const float y = to_f32(x[j]);
-                        count += __builtin_popcountll(__ballot(y >= least && score_key(y, j) >= c));
-                    }
-                    __syncthreads();
-                    if (threadIdx.x == 0) s_n = 0;
-                    __syncthreads();
-                    if (lane == 0) atomicAdd(&s_n, count);
-                    __syncthreads();
-                    return s_n;
-                });
-                __syncthreads();
-                if (threadIdx.x == 0) s_n = 0;
-                __syncthreads();
-                for (unsigned j = j0 + threadIdx.x; j < j1; j += NT) {
-                    const float y = to_f32(x[j]);
-                    if (y >= least && score_key(y, j) >= reach) s_list[atomicAdd(&s_n, 1)] = score_key(y, j);
-                }
-                __syncthreads();
-            }
-        } else {
-            __syncthreads();
-        }
-        if (wave == 0) {
-            r.s = wave_reduce(lane < WAVES ? s_s[lane] : 0.0f, SumOf());
-            r.u = wave_reduce(lane < WAVES ? s_u[lane] : 0.0f, SumOf());
-            if (lane == 0) {
-                if (a.pieces == 1) {
-                    const int t = a.target ? a.target[row] : -1;
-                    const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
-                    logprob_write(a, row, r, has_t ? to_f32(x[t]) : 0.0f, has_t);
-                } else
-                    a.part[work] = r;
-            }
+            s += es;
+            u += eu;
             if (a.top) {
-                const int n = keep_best(s_list, s_n, a.top, lane);
-                __builtin_amdgcn_wave_barrier();
-                const unsigned long long key = lane < n ? s_list[lane] : 0;
-                const int place = key_place(key, n);
-                if (a.pieces == 1) {
-                    if (lane < n && place < a.top) logprob_write_top(a, row, r, place, key);
-                    if (lane >= n && lane < a.top) logprob_write_top(a, row, r, lane, 0);
-                } else {
-                    if (lane < n && place < a.top) a.part_top[work * a.top + place] = key;
-                    if (lane >= n && lane < a.top) a.part_top[work * a.top + lane] = 0;
+                if (step == 0) best.least = reached_by(top, a.top);
+                if (__ballot(top >= best.least)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) best.offer(v[e], j0 - off + ((step * U + e / V) * 64 + lane) * V + e % V, a.top, lane);
                 }
             }
+#pragma unroll
+            for (int q = 0; q < U; q++) cur[q] = next[q];
         }
-        __syncthreads();   // before the next row's s_group, s_n and s_list
+        LogprobPart r;
+        r.m = wave_reduce(m, MaxOf());
+        // a reference of -inf: every score ruled out, or NaN in s
+        const float d = ref == kNegInf ? 0.0f : ref - r.m, w = __builtin_amdgcn_exp2f(d * c);
+        s = wave_reduce(s, SumOf());
+        u = wave_reduce(u, SumOf());
+        r.s = w * s;
+        r.u = w * fmaf(fmaxf(d, least_t), s, u);
+        const float log_s = log_of_sum(r.s);
+        if (lane == 0) {
+            if (a.pieces == 1) {
+                const int t = a.target ? a.target[row] : -1;
+                const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
+                logprob_write(a, row, r, log_s, has_t ? to_f32(x[t]) : 0.0f, has_t);
+            } else
+                a.part[work] = r;
+        }
+        if (!a.top) continue;
+        if (best.n > 64) best.shrink(a.top, lane);
+        __builtin_amdgcn_wave_barrier();
+        if (a.pieces == 1)
+            logprob_write_list(a, row, r, log_s, best.list, best.n, lane);
+        else {
+            const unsigned long long key = lane < best.n ? best.list[lane] : 0;
+            const int place = key_place(key, best.n);
+            if (lane < best.n && place < a.top) a.part_top[work * a.top + place] = key;
+            if (lane >= best.n && lane < a.top) a.part_top[work * a.top + lane] = 0;
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
 // ---- the pieces of a row joined, a wave per row ----
 __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int type)
 {
-    __shared__ unsigned long long s_list[kCandidates];
+    __shared__ unsigned long long s_list[64];
     const int lane = threadIdx.x;
     for (unsigned long long row = blockIdx.x; row < a.n; row += gridDim.x) {
+        // the first 1024 keys of the pieces' lists: asked for before the sums are joined
+        const unsigned long long *keys = a.part_top + row * a.pieces * a.top, all = (unsigned long long)a.pieces * a.top;
+        unsigned long long k[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) k[i] = 64u * i + lane < all ? keys[64 * i + lane] : 0;
         const LogprobPart *part = a.part + row * a.pieces;
+        const int t = a.target ? a.target[row] : -1;
+        const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
+        float xt = 0.0f;
+        if (has_t) {
+            const unsigned long long at = row * a.ld + (unsigned)t;
+            xt = type == 0 ? ((const float *)a.x)[at] : type == 1 ? to_f32(((const f16_t *)a.x)[at]) : to_f32(((const bf16_t *)a.x)[at]);
+        }
         LogprobPart r;
         float m = kNegInf;
         for (unsigned p = lane; p < a.pieces; p += 64) m = fmaxf(m, part[p].m);
@@ -394,62 +419,45 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
         }
         r.s = wave_reduce(s, SumOf());
         r.u = wave_reduce(u, SumOf());
-        if (lane == 0) {
-            const int t = a.target ? a.target[row] : -1;
-            const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
-            float xt = 0.0f;
-            if (has_t) {
-                const unsigned long long at = row * a.ld + (unsigned)t;
-                xt = type == 0 ? ((const float *)a.x)[at] : type == 1 ? to_f32(((const f16_t *)a.x)[at]) : to_f32(((const bf16_t *)a.x)[at]);
-            }
-            logprob_write(a, row, r, xt, has_t);
-        }
+        const float log_s = log_of_sum(r.s);
+        if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
-        // the pieces' lists through LDS, as many at a time as fit beside the best so far
-        const unsigned long long *keys = a.part_top + row * a.pieces * a.top, all = (unsigned long long)a.pieces * a.top;
-        int n = 0;
-        for (unsigned long long k0 = 0; k0 < all;) {
-            const int more = (int)min(all - k0, (unsigned long long)(kCandidates - n));
-            int kept = n;
-            for (int i = 0; i < more; i += 64) {
-                const unsigned long long key = i + lane < more ? keys[k0 + i + lane] : 0, in = __ballot(key != 0);
-                if (key) s_list[kept + __builtin_popcountll(in & ((1ull << lane) - 1))] = key;
-                kept += __builtin_popcountll(in);
+        unsigned long long border;
+        int n = keep_best(k, a.top, lane, s_list, border);
+        for (unsigned long long k0 = 1024; k0 < all; k0 += 960) {   // more pieces: with the best so far in the first place
+            __builtin_amdgcn_wave_barrier();
+            k[0] = lane < n ? s_list[lane] : 0;
+#pragma unroll
+            for (int i = 1; i < 16; i++) {
+                const unsigned long long at = k0 + 64 * (i - 1) + lane;
+                k[i] = at < all ? keys[at] : 0;
             }
-            k0 += more;
             __builtin_amdgcn_wave_barrier();
-            n = keep_best(s_list, kept, a.top, lane);
-            __builtin_amdgcn_wave_barrier();
+            n = keep_best(k, a.top, lane, s_list, border);
         }
-        const unsigned long long key = lane < n ? s_list[lane] : 0;
-        const int place = key_place(key, n);
-        if (lane < n && place < a.top) logprob_write_top(a, row, r, place, key);
-        if (lane >= n && lane < a.top) logprob_write_top(a, row, r, lane, 0);
+        __builtin_amdgcn_wave_barrier();
+        logprob_write_list(a, row, r, log_s, s_list, n, lane);
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-// How a call's rows are cut: lanes and scores a lane of a workgroup (0 lanes: a wave per row), pieces of a row and their length.
+// How a call's rows are cut: scores a lane of a wave that holds a whole row (0: rows are streamed), pieces of a row and their length.
 struct LogprobPlan {
-    int threads, each;
+    int each;
     unsigned pieces, piece_len;
     size_t work;   // bytes
 };
+constexpr size_t kWavesWanted = 4096, kLeastPiece = 4096;
 inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
 {
-    LogprobPlan p = {0, 1, 1, (unsigned)c, 0};
+    LogprobPlan p = {0, 1, (unsigned)c, 0};
     if (c <= 1024) {
-        while (64 * p.each < (int)c) p.each *= 2;
+        p.each = (int)((c + 63) / 64);
         return p;
     }
-    // rows to spare for every CU: the shortest workgroup that holds a row, or the longest; otherwise short pieces, so that the rows
-    // at hand reach more CUs (a piece loses up to 7 places to alignment)
-    const bool many = n * ((c + 32759) / 32760) >= 256;
-    p.threads = c <= 4088 || !many ? 256 : c <= 8184 ? 256 : c <= 16376 ? 512 : 1024;
-    p.each = p.threads == 256 && (c <= 4088 || !many) ? 16 : 32;
-    const size_t room = (size_t)p.threads * p.each - 8;
-    p.pieces = (unsigned)((c + room - 1) / room);
-    p.piece_len = (unsigned)(((c + p.pieces - 1) / p.pieces + 7) / 8 * 8);
+    // pieces while the rows alone are too few waves for the chip
+    const size_t pieces = std::min((kWavesWanted + n - 1) / std::max<size_t>(n, 1), (c + kLeastPiece - 1) / kLeastPiece);
+    p.piece_len = (unsigned)(((c + pieces - 1) / pieces + 7) / 8 * 8);
     p.pieces = (unsigned)((c + p.piece_len - 1) / p.piece_len);
     if (p.pieces > 1) p.work = n * p.pieces * (size_t)top * 8 + (n * p.pieces * sizeof(LogprobPart) + 15) / 16 * 16;
     return p;

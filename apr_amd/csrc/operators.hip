@@ -66,20 +66,32 @@ void with_type(int dtype, F f)
 template <typename T>
 void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPlan &p)
 {
-    if (!p.threads) {
+    if (p.each) {
         const dim3 grid((unsigned)std::min<unsigned long long>((a.n + 3) / 4, kMostBlocks)), block(256);
-        if (p.each == 1) hipLaunchKernelGGL((logprob_wave_kernel<T, 1>), grid, block, 0, v.stream, a);
-        else if (p.each == 2) hipLaunchKernelGGL((logprob_wave_kernel<T, 2>), grid, block, 0, v.stream, a);
-        else if (p.each == 4) hipLaunchKernelGGL((logprob_wave_kernel<T, 4>), grid, block, 0, v.stream, a);
-        else if (p.each == 8) hipLaunchKernelGGL((logprob_wave_kernel<T, 8>), grid, block, 0, v.stream, a);
-        else hipLaunchKernelGGL((logprob_wave_kernel<T, 16>), grid, block, 0, v.stream, a);
-        return;
+        const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, v.stream, a); };
+        switch (p.each) {   // scores a lane: what a row has beyond them is computed for nothing
+        case 1: return launch(logprob_wave_kernel<T, 1>);
+        case 2: return launch(logprob_wave_kernel<T, 2>);
+        case 3: return launch(logprob_wave_kernel<T, 3>);
+        case 4: return launch(logprob_wave_kernel<T, 4>);
+        case 5: return launch(logprob_wave_kernel<T, 5>);
+        case 6: return launch(logprob_wave_kernel<T, 6>);
+        case 7: return launch(logprob_wave_kernel<T, 7>);
+        case 8: return launch(logprob_wave_kernel<T, 8>);
+        case 9: return launch(logprob_wave_kernel<T, 9>);
+        case 10: return launch(logprob_wave_kernel<T, 10>);
+        case 11: return launch(logprob_wave_kernel<T, 11>);
+        case 12: return launch(logprob_wave_kernel<T, 12>);
+        case 13: return launch(logprob_wave_kernel<T, 13>);
+        case 14: return launch(logprob_wave_kernel<T, 14>);
+        case 15: return launch(logprob_wave_kernel<T, 15>);
+        default: return launch(logprob_wave_kernel<T, 16>);
+        }
     }
-    const dim3 grid((unsigned)std::min<unsigned long long>(a.n * a.pieces, kMostBlocks));
-    if (p.threads == 1024) hipLaunchKernelGGL((logprob_block_kernel<T, 1024, 32>), grid, dim3(1024), 0, v.stream, a);
-    else if (p.threads == 512) hipLaunchKernelGGL((logprob_block_kernel<T, 512, 32>), grid, dim3(512), 0, v.stream, a);
-    else if (p.each == 32) hipLaunchKernelGGL((logprob_block_kernel<T, 256, 32>), grid, dim3(256), 0, v.stream, a);
-    else hipLaunchKernelGGL((logprob_block_kernel<T, 256, 16>), grid, dim3(256), 0, v.stream, a);
+    // few waves: one in a workgroup, so that they spread over the CUs
+    const unsigned long long works = a.n * a.pieces;
+    const unsigned waves = works < 4ull * v.n_cus ? 1 : 4;
+    hipLaunchKernelGGL(logprob_stream_kernel<T>, dim3((unsigned)std::min<unsigned long long>((works + waves - 1) / waves, kMostBlocks)), dim3(64 * waves), 0, v.stream, a);
 }
 
 // Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.

@@ -192,8 +192,8 @@ def test_offsets_beyond_32_bits(eng):
     x = torch.as_strided(store, (3, c), (ld, 1))
     src, t = rows(3, c, torch.bfloat16, 8)
     x.copy_(src)
-    want, got = run(eng, src, t, 5), run(eng, x, t, 5)
-    assert all(torch.equal(got[k], want[k]) for k in want)
+    assert torch.equal(x, src)
+    got = check(eng, x, t, 5)    # not src's bits: a row that begins elsewhere in a 16-byte unit is summed in another order
     stat, ent = got["stat"].contiguous(), got["entropy"].contiguous()
     g = torch.full((3,), -0.5, device=dev())
     a, b = torch.empty(3, c, device=dev(), dtype=torch.bfloat16), x

@@ -471,27 +471,62 @@ struct LogprobGradArgs {
     float scale;
     const int32_t *target;
     const float *stat, *entropy, *g_logprob, *g_entropy;
+    unsigned pieces, piece_units;   // a row's units of 16 bytes (of grad) that a wave takes
 };
 
-// One workgroup per row; an element is read before the same thread writes it, so grad may be x.
-template <typename T>
+// A wave per row, or per piece of one.  Reads and writes every score once; an element is read before its place is written by the same
+// lane, so grad may be x.  Stores are whole 16-byte units of grad, wherever its rows begin (what a row has before its first
+// and behind its last whole unit goes element by element); the loads follow them at whatever alignment x has then, which the hardware takes.
+// p = exp2(scale log2 e (x - m) - log2 e log s): x - m is exact for the scores that matter, the rest rounds once.
+template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(256) void logprob_grad_kernel(LogprobGradArgs a)
 {
-    for (unsigned long long row = blockIdx.x; row < a.n; row += gridDim.x) {
+    constexpr int V = 16 / (int)sizeof(T);
+    typedef T txv __attribute__((ext_vector_type(V)));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const unsigned long long works = a.n * a.pieces;
+    const float c = a.scale * kLog2E;
+    for (unsigned long long work = (unsigned long long)blockIdx.x * waves + wave; work < works; work += (unsigned long long)gridDim.x * waves) {
+        const unsigned long long row = a.pieces == 1 ? work : work / a.pieces;
+        const unsigned piece = (unsigned)(work - row * a.pieces);
         const T *x = (const T *)a.x + row * a.ld;
         T *grad = (T *)a.grad + row * a.ld_grad;
+        // the row: `head` elements up to grad's first 16-byte unit, whole units, `tail` elements
+        const unsigned off = (unsigned)(((unsigned long long)grad & 15) / sizeof(T));
+        const unsigned head = off ? min(V - off, a.n_labels) : 0, n_units = (a.n_labels - head) / V, tail = a.n_labels - head - n_units * V;
+        const unsigned w0 = piece * a.piece_units, w1 = min(w0 + a.piece_units, n_units);
         const float m = a.stat[2 * row], log_s = a.stat[2 * row + 1];
         const int t = a.target ? a.target[row] : -1;
-        const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
-        const float g = has_t && a.g_logprob ? a.g_logprob[row] : 0.0f;
-        const float h = a.g_entropy ? a.g_entropy[row] : 0.0f;
-        const float ent = a.g_entropy ? a.entropy[row] : 0.0f;
-        for (unsigned j = threadIdx.x; j < a.n_labels; j += 256) {
-            const float l = m == kNegInf ? kNegInf : a.scale * (to_f32(x[j]) - m) - log_s;
-            const float p = __expf(l);
-            float r = -p * (g + h * (fmaxf(l, -200.0f) + ent));
-            if (has_t && j == (unsigned)t && m != kNegInf) r += g;
-            grad[j] = from_f32<T>(a.scale * r);
+        const bool empty = m == kNegInf, has_t = t >= 0 && (unsigned)t < a.n_labels && !empty;
+        const float g = has_t && a.g_logprob ? a.g_logprob[row] : 0.0f, h = ENTROPY ? a.g_entropy[row] : 0.0f, ent = ENTROPY ? a.entropy[row] : 0.0f;
+        const float gs = -a.scale * g, hs = -a.scale * h, ls2 = log_s * kLog2E;
+        const auto one = [&](float v) {
+            const float l2 = fmaf(v - m, c, -ls2), p = __builtin_amdgcn_exp2f(l2);
+            float f = gs;
+            if (ENTROPY) f = fmaf(hs, fmaf(fmaxf(l2, -300.0f), 0.69314718055994530942f, ent), gs);   // exp2(-300) = 0; no 0 * inf
+            return empty ? 0.0f : p * f;
+        };
+        const unsigned tu = has_t && (unsigned)t >= head ? ((unsigned)t - head) / V : 0xFFFFFFFFu, tv = ((unsigned)t - head) % V;
+        const T *xb = x + head;
+        T *gb = grad + head;
+#pragma unroll 4
+        for (unsigned w = w0 + lane; w < w1; w += 64) {
+            txv v, r;
+            __builtin_memcpy(&v, xb + (unsigned long long)w * V, 16);
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) f[i] = one(to_f32(v[i]));
+            if (w == tu) {
+#pragma unroll
+                for (int i = 0; i < V; i++) f[i] -= i == (int)tv ? gs : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) r[i] = from_f32<T>(f[i]);
+            __builtin_nontemporal_store(r, (txv *)(gb + (unsigned long long)w * V));
+        }
+        if (piece == 0) {
+            const unsigned e = (unsigned)lane < head ? lane : a.n_labels - tail + (lane - 32);
+            if ((unsigned)lane < head || (lane >= 32 && lane - 32 < (int)tail)) grad[e] = from_f32<T>(one(to_f32(x[e])) - (has_t && e == (unsigned)t ? gs : 0.0f));
         }
     }
 }

@@ -94,6 +94,25 @@ void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPla
     hipLaunchKernelGGL(logprob_stream_kernel<T>, dim3((unsigned)std::min<unsigned long long>((works + waves - 1) / waves, kMostBlocks)), dim3(64 * waves), 0, v.stream, a);
 }
 
+// The smallest group of lanes that holds a row's 16-byte units in registers
+template <typename T>
+void launch_rowquant(const EngineView &v, const RowQuantArgs &a)
+{
+    constexpr unsigned V = 16 / sizeof(T);
+    const bool whole = aligned(a.x, 16) && a.ld % V == 0;
+    const unsigned long long units = (a.k + (whole ? 0ull : V - 1) + V - 1) / V;   // a row may begin inside a unit
+    const auto launch = [&](auto kernel, unsigned rows, unsigned threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<unsigned long long>((a.n + rows - 1) / rows, kMostBlocks)), dim3(threads), 0, v.stream, a);
+    };
+    if (units <= 64) launch(rowquant_kernel<T, 1, 1>, 4, 256);
+    else if (units <= 128) launch(rowquant_kernel<T, 1, 2>, 4, 256);
+    else if (units <= 256) launch(rowquant_kernel<T, 1, 4>, 4, 256);
+    else if (units <= 512) launch(rowquant_kernel<T, 1, 8>, 4, 256);
+    else if (units <= 1024) launch(rowquant_kernel<T, 4, 4>, 1, 256);
+    else if (units <= 2048) launch(rowquant_kernel<T, 4, 8>, 1, 256);
+    else launch(rowquant_kernel<T, 16, 8>, 1, 1024);
+}
+
 // Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.
 template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN>
 void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
@@ -190,9 +209,16 @@ int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_l
     LogprobGradArgs a;
     a.x = d_logits; a.grad = d_grad; a.n = n; a.ld = ld; a.ld_grad = ld_grad; a.n_labels = (unsigned)n_labels; a.scale = (float)scale;
     a.target = d_target; a.stat = d_stat; a.entropy = d_entropy; a.g_logprob = d_g_logprob; a.g_entropy = d_g_entropy;
+    // pieces of 512 units or more, while the rows alone are too few waves for the chip
+    const size_t units = std::max<size_t>(n_labels * element_size(dtype) / 16, 1);
+    const size_t pieces = std::max<size_t>(1, std::min((2 * kWavesWanted + n - 1) / n, units / 512));
+    a.piece_units = (unsigned)((units + pieces - 1) / pieces);
+    a.pieces = (unsigned)((units + a.piece_units - 1) / a.piece_units);
     return on_engine(e, me, [&](const EngineView &v) {
+        const dim3 grid((unsigned)std::min<size_t>((n * a.pieces + 3) / 4, kMostBlocks)), block(256);
         with_type(dtype, [&](auto *p) {
-            hipLaunchKernelGGL(logprob_grad_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(256), 0, v.stream, a);
+            if (a.g_entropy) hipLaunchKernelGGL((logprob_grad_kernel<APR_TYPE_OF(p), true>), grid, block, 0, v.stream, a);
+            else hipLaunchKernelGGL((logprob_grad_kernel<APR_TYPE_OF(p), false>), grid, block, 0, v.stream, a);
         });
     });
 }
@@ -209,9 +235,7 @@ int apr_quantize_rows_device(apr_engine *e, int dtype, const void *d_x, size_t n
     RowQuantArgs a;
     a.x = d_x; a.q = d_q; a.scale = d_scale; a.n = n; a.ld = ld; a.ld_q = ld_q; a.k = (unsigned)k;
     return on_engine(e, me, [&](const EngineView &v) {
-        with_type(dtype, [&](auto *p) {
-            hipLaunchKernelGGL(rowquant_kernel<APR_TYPE_OF(p)>, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(256), 0, v.stream, a);
-        });
+        with_type(dtype, [&](auto *p) { launch_rowquant<APR_TYPE_OF(p)>(v, a); });
     });
 }
 

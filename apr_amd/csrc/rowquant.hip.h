@@ -31,27 +31,84 @@ struct RowQuantArgs {
     unsigned k;
 };
 
-// One workgroup per row.
-template <typename T>
-__global__ __launch_bounds__(256) void rowquant_kernel(RowQuantArgs a)
+// G waves per row, U units of 16 bytes a lane in registers, read once (a row that is longer than that is read twice).  HBM-bound.  16-byte loads
+// begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is); what does not belong
+// to the row counts as 0 and is not written.  A lane writes the 4 or 8 values of its unit together, at whatever alignment they have.
+template <typename T, int G, int U>
+__global__ __launch_bounds__(G == 1 ? 256 : G * 64) void rowquant_kernel(RowQuantArgs a)
 {
-    __shared__ uint32_t s_part[4];
-    for (unsigned long long row = blockIdx.x; row < a.n; row += gridDim.x) {
+    constexpr int V = 16 / (int)sizeof(T), LANES = G * 64;
+    typedef T txv __attribute__((ext_vector_type(V)));
+    typedef int8_t qxv __attribute__((ext_vector_type(V)));
+    __shared__ uint32_t s_part[2][G];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), me = G == 1 ? lane : (int)threadIdx.x;
+    constexpr unsigned ROWS = G == 1 ? 4 : 1;   // rows that a workgroup has at hand
+    int flip = 0;
+    for (unsigned long long row = (unsigned long long)blockIdx.x * ROWS + (G == 1 ? wave : 0); row < a.n; row += (unsigned long long)gridDim.x * ROWS) {
         const T *x = (const T *)a.x + row * a.ld;
+        int8_t *q = a.q + row * a.ld_q;
+        const unsigned off = (unsigned)(((unsigned long long)x & 15) / sizeof(T));
+        const txv *units = (const txv *)(x - off);
+        const unsigned long long len = (unsigned long long)a.k + off;
+        const unsigned n_units = (unsigned)((len + V - 1) / V);
+        txv v[U];
         // magnitudes as bit patterns: NaN above infinity above every number
         uint32_t most = 0;
-        for (unsigned j = threadIdx.x; j < a.k; j += 256) most = max(most, __builtin_bit_cast(uint32_t, to_f32(x[j])) & 0x7FFFFFFFu);
+        const auto load = [&](unsigned base) {
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const unsigned w = base + i * LANES + me;
+                if (w < n_units) v[i] = units[w];
+                else v[i] = (T)0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const unsigned w = base + i * LANES + me;
+                if (w == 0 || w == n_units - 1) {
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        if ((unsigned long long)w * V + e < off || (unsigned long long)w * V + e >= len) v[i][e] = (T)0.0f;
+                }
+            }
+        };
+        for (unsigned base = 0; base < n_units; base += U * LANES) {
+            load(base);
+#pragma unroll
+            for (int i = 0; i < U; i++)
+#pragma unroll
+                for (int e = 0; e < V; e++) most = max(most, __builtin_bit_cast(uint32_t, to_f32(v[i][e])) & 0x7FFFFFFFu);
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = most;
-        __syncthreads();
-        most = max(max(s_part[0], s_part[1]), max(s_part[2], s_part[3]));
+        if (G > 1) {
+            if (lane == 0) s_part[flip][wave] = most;   // two sets: the next row's may be written while this one's are read
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < G; w++) most = max(most, s_part[flip][w]);
+            flip ^= 1;
+        }
         const float am = __builtin_bit_cast(float, most);
         const bool bad = most >= 0x7F800000u, none = bad || am < kLeastRow;
         const double inv = none ? 0.0 : 127.0 / (double)am;
-        if (threadIdx.x == 0) a.scale[row] = bad ? __builtin_nanf("") : none ? 0.0f : am / 127.0f;
-        for (unsigned j = threadIdx.x; j < a.k; j += 256) a.q[row * a.ld_q + j] = none ? (int8_t)0 : (int8_t)quantize_one(to_f32(x[j]), inv);
+        if (me == 0) a.scale[row] = bad ? __builtin_nanf("") : none ? 0.0f : am / 127.0f;
+        for (unsigned base = 0; base < n_units; base += U * LANES) {
+            if (n_units > U * LANES) load(base);   // otherwise the row is still there
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const unsigned w = base + i * LANES + me;
+                if (w >= n_units) continue;
+                qxv r;
+#pragma unroll
+                for (int e = 0; e < V; e++) r[e] = none ? (int8_t)0 : (int8_t)quantize_one(to_f32(v[i][e]), inv);
+                const long long j = (long long)w * V - off;
+                if (j >= 0 && j + V <= (long long)a.k) __builtin_memcpy(q + j, &r, V);
+                else {
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        if (j + e >= 0 && j + e < (long long)a.k) q[j + e] = r[e];
+                }
+            }
+        }
     }
 }
 

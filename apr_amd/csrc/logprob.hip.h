@@ -36,25 +36,22 @@ __device__ __forceinline__ float key_score(unsigned long long key)
 __device__ __forceinline__ int key_label(unsigned long long key) { return (int)~(uint32_t)key; }
 
 // ---- reductions of a wave (64 lanes) ----
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float lane_move(float v)
-{
-    const int b = __builtin_bit_cast(int, v);
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, CTRL, ROWS, 0xf, false));
-}
+// Another lane's value, by a pattern in which every lane has a source: folds into the instruction that uses it
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)); }
 // over the four lanes of a quad, and over the sixteen of a row: every lane has the result
 template <typename F>
 __device__ __forceinline__ float quad_reduce(float v, F f)
 {
-    v = f(v, lane_move<0xB1, 0xf>(v));   // lane ^ 1
-    return f(v, lane_move<0x4E, 0xf>(v));   // lane ^ 2
+    v = f(v, lane_move<0xB1>(v));   // lane ^ 1
+    return f(v, lane_move<0x4E>(v));   // lane ^ 2
 }
 template <typename F>
 __device__ __forceinline__ float row_reduce(float v, F f)
 {
     v = quad_reduce(v, f);
-    v = f(v, lane_move<0x141, 0xf>(v));   // mirrored within eight
-    return f(v, lane_move<0x140, 0xf>(v));   // mirrored within sixteen
+    v = f(v, lane_move<0x141>(v));   // mirrored within eight
+    return f(v, lane_move<0x140>(v));   // mirrored within sixteen
 }
 // over all lanes, from row results; wave-uniform
 template <typename F>
@@ -115,7 +112,7 @@ __device__ __forceinline__ void logprob_write(const LogprobArgs &a, unsigned lon
         a.stat[2 * row] = bad ? kNaN : r.m;
         a.stat[2 * row + 1] = bad ? kNaN : log_s;
     }
-    if (a.entropy) a.entropy[row] = bad ? kNaN : empty ? 0.0f : fmaxf(log_s - a.scale * (r.u / r.s), 0.0f);
+    if (a.entropy) a.entropy[row] = bad ? kNaN : empty ? 0.0f : fmaxf(log_s - a.scale * (r.u * __builtin_amdgcn_rcpf(r.s)), 0.0f);
     if (a.logprob) a.logprob[row] = !has_target ? 0.0f : bad ? kNaN : empty ? kNegInf : a.scale * (x_target - r.m) - log_s;
 }
 __device__ __forceinline__ void logprob_write_top(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, int place, unsigned long long key)
@@ -155,11 +152,14 @@ __device__ __forceinline__ int key_place(unsigned long long key, int n)
     return place;
 }
 
-// Of the wave's keys k[0..N-1] (0: none) at most 64 that hold the best `top` are left in `list` (LDS); returns how many, and in
+// Lanes below this one in a mask
+__device__ __forceinline__ int below(unsigned long long mask) { return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0)); }
+
+// Of the wave's keys k[0..N-1] (0: none) at most 64 that hold the best `top` are put at places 0, 1, ..; returns how many, and in
 // `border` a key that none of the dropped ones reaches.  Counting reached candidates of a binary search: 16 bits of the score first, and
 // if equal scores leave more than 64, all other bits, which ends at the `top`-th key itself, as every key is there once.
-template <int N>
-__device__ __forceinline__ int keep_best(const unsigned long long (&k)[N], int top, int lane, unsigned long long *list, unsigned long long &border)
+template <int N, typename F>
+__device__ __forceinline__ int keep_best(const unsigned long long (&k)[N], int top, unsigned long long &border, F put)
 {
     uint32_t t = 0;
 #pragma unroll
@@ -187,53 +187,91 @@ __device__ __forceinline__ int keep_best(const unsigned long long (&k)[N], int t
     for (int i = 0; i < N; i++) {
         const bool in = k[i] >= reach && k[i];
         const unsigned long long mask = __ballot(in);
-        if (in) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = k[i];
+        if (in) put(n + below(mask), k[i]);
         n += __builtin_popcountll(mask);
     }
     border = reach;
     return n;
 }
 
-// The alternatives of a row from at most 64 keys in `list`
-__device__ __forceinline__ void logprob_write_list(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, const unsigned long long *list, int n, int lane)
+// The alternatives of a row from at most 64 keys, one each of the first n lanes
+__device__ __forceinline__ void logprob_write_list(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, unsigned long long key, int n, int lane)
 {
-    const unsigned long long key = lane < n ? list[lane] : 0;
     const int place = key_place(key, n);
     if (lane < n && place < a.top) logprob_write_top(a, row, r, log_s, place, key);
     if (lane >= n && lane < a.top) logprob_write_top(a, row, r, log_s, lane, 0);
 }
 
-// A wave's candidates for the alternatives, collected in LDS as its scores come by, 64 lanes at a time.  Taken are scores of at least
-// `least` whose key passes `border`; when the list is full, the best are kept and both rise.
+// A wave's candidates for the alternatives, collected in LDS as its scores come by.  Taken are scores of at least `least`; when the list
+// is full, the best are kept and `least` rises.  If equal scores still are too many, they are taken one by one, and only those whose key
+// passes `border`.  An entry is the score's bits and the label; keys are made of them when the list is looked at, which is much rarer.
 constexpr int kList = 128;
 struct Candidates {
-    unsigned long long *list, border = 0;
+    uint2 *list;
+    unsigned long long border = 0;
     int n = 0;
     float least = __builtin_inff();
-    __device__ __forceinline__ explicit Candidates(unsigned long long *l) : list(l) {}
+    __device__ __forceinline__ explicit Candidates(uint2 *l) : list(l) {}
+    __device__ __forceinline__ unsigned long long key_at(int i) const
+    {
+        if (i >= n) return 0;
+        const uint2 v = list[i];
+        return score_key(__builtin_bit_cast(float, v.x), v.y);
+    }
     __device__ __forceinline__ void shrink(int top, int lane)
     {
         __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
         unsigned long long k[kList / 64];
 #pragma unroll
-        for (int i = 0; i < kList / 64; i++) k[i] = 64 * i + lane < n ? list[64 * i + lane] : 0;
+        for (int i = 0; i < kList / 64; i++) k[i] = key_at(64 * i + lane);
         __builtin_amdgcn_wave_barrier();
-        n = keep_best(k, top, lane, list, border);
+        n = keep_best(k, top, border, [&](int at, unsigned long long key) { list[at] = make_uint2(__builtin_bit_cast(uint32_t, key_score(key)), (unsigned)key_label(key)); });
         least = fmaxf(least, key_score(border));
         __builtin_amdgcn_wave_barrier();
     }
-    // one score of every lane
-    __device__ __forceinline__ void offer(float v, unsigned label, int top, int lane)
+    // N scores of every lane, their labels label(i), and the same score again from memory
+    template <int N, typename L, typename M>
+    __device__ __forceinline__ void offer(const float (&v)[N], int top, int lane, L label, M again)
     {
-        if (!__ballot(v >= least)) return;
-        const unsigned long long key = score_key(v, label);
-        unsigned long long mask = __ballot(v >= least && key >= border);
-        if (n + __builtin_popcountll(mask) > kList) {   // then n > 64, and no more than 64 are left
-            shrink(top, lane);
-            mask = __ballot(v >= least && key >= border);
+        for (bool full = false;; full = true) {
+            int more = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) more += __builtin_popcountll(__ballot(v[i] >= least));
+            if (n + more <= kList) {
+                if (more) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const unsigned long long mask = __ballot(v[i] >= least);
+                        if (!mask) continue;
+                        if (mask >> lane & 1) list[n + below(mask)] = make_uint2(__builtin_bit_cast(uint32_t, v[i]), label(i));
+                        n += __builtin_popcountll(mask);
+                    }
+                }
+                return;
+            }
+            if (full) break;
+            if (n > 0) shrink(top, lane);
         }
-        if (mask >> lane & 1) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = key;
-        n += __builtin_popcountll(mask);
+        // a loop over memory: this is rare, and unrolled over the registers it would take more of them
+        for (int i = 0; i < N; i++) {
+            const float y = again(i);
+            unsigned long long mask = __ballot(y >= least && score_key(y, label(i)) >= border);
+            if (n + __builtin_popcountll(mask) > kList) {   // then n > 64, and no more than 64 are left
+                shrink(top, lane);
+                mask = __ballot(y >= least && score_key(y, label(i)) >= border);
+            }
+            if (mask >> lane & 1) list[n + below(mask)] = make_uint2(__builtin_bit_cast(uint32_t, y), label(i));
+            n += __builtin_popcountll(mask);
+        }
+    }
+    // at most 64 keys, one a lane (0: none)
+    __device__ __forceinline__ unsigned long long finish(int top, int lane)
+    {
+        if (n > 64) shrink(top, lane);
+        __builtin_amdgcn_wave_barrier();
+        const unsigned long long key = key_at(lane);
+        __builtin_amdgcn_wave_barrier();
+        return key;
     }
 };
 
@@ -243,16 +281,14 @@ struct Candidates {
 template <typename T, int E>
 __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
 {
-    __shared__ unsigned long long s_list[4][kList];
+    __shared__ uint2 s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (unsigned long long row = (unsigned long long)blockIdx.x * 4 + wave; row < a.n; row += (unsigned long long)gridDim.x * 4) {
         const T *x = (const T *)a.x + row * a.ld;
-        const int t = a.target ? a.target[row] : -1;
-        const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
-        const float xt = has_t ? to_f32(x[t]) : 0.0f;
         float v[E], best = kNegInf;
 #pragma unroll
         for (int i = 0; i < E; i++) v[i] = i < E - 1 || 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf;
+        const int t = a.target ? __builtin_amdgcn_readfirstlane(a.target[row]) : -1;
 #pragma unroll
         for (int i = 0; i < E; i++) best = fmaxf(best, v[i]);
         LogprobPart r;
@@ -263,16 +299,18 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         r.s = wave_reduce(sum.s, SumOf());
         r.u = wave_reduce(sum.u, SumOf());
         const float log_s = log_of_sum(r.s);
+        const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
+        float xt = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            if (has_t && t >> 6 == i) xt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[i]), t & 63));
         if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
         Candidates c(s_list[wave]);
         c.least = reached_by(best, a.top);
-#pragma unroll
-        for (int i = 0; i < E; i++) c.offer(v[i], 64 * i + lane, a.top, lane);
-        if (c.n > 64) c.shrink(a.top, lane);
-        __builtin_amdgcn_wave_barrier();
-        logprob_write_list(a, row, r, log_s, c.list, c.n, lane);
-        __builtin_amdgcn_wave_barrier();
+        c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
+        const unsigned long long key = c.finish(a.top, lane);
+        logprob_write_list(a, row, r, log_s, key, c.n, lane);
     }
 }
 
@@ -285,12 +323,13 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
 // what does not belong to the piece counts as ruled out.
 constexpr float kGap = 8.0f;
 
-template <typename T>
-__global__ __launch_bounds__(256, 8) void logprob_stream_kernel(LogprobArgs a)
+// TOP: with alternatives, whose code takes registers (98 of them: five waves a SIMD instead of eight).
+template <typename T, bool TOP>
+__global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(LogprobArgs a)
 {
     constexpr int V = 16 / (int)sizeof(T), U = 16 / V;
     typedef T txv __attribute__((ext_vector_type(V)));
-    __shared__ unsigned long long s_list[4][kList];
+    __shared__ uint2 s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const unsigned long long works = a.n * a.pieces;
     const float c = a.scale * kLog2E, gap = kGap / a.scale, least_t = -200.0f / a.scale;
@@ -301,6 +340,7 @@ __global__ __launch_bounds__(256, 8) void logprob_stream_kernel(LogprobArgs a)
         const unsigned off = (unsigned)(((unsigned long long)(x + j0) & 15) / sizeof(T));
         const txv *units = (const txv *)(x + j0 - off);
         const unsigned len = j1 - j0 + off, n_units = (len + V - 1) / V, steps = (n_units + 64 * U - 1) / (64 * U);
+        const unsigned keep = len - (n_units - 1) * V;   // elements of the last unit
         txv cur[U], next[U];
         const auto load = [&](txv(&to)[U], unsigned step) {
 #pragma unroll
@@ -318,11 +358,16 @@ __global__ __launch_bounds__(256, 8) void logprob_stream_kernel(LogprobArgs a)
             float v[16], top = kNegInf;
 #pragma unroll
             for (int e = 0; e < 16; e++) v[e] = to_f32(cur[e / V][e % V]);
-            if (step == 0 || step == steps - 1) {
+            if (step == 0 && off) {   // the first unit is lane 0's
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const unsigned at = ((step * U + e / V) * 64 + lane) * V + e % V;
-                    if (at < off || at >= len) v[e] = kNegInf;
+                for (int i = 0; i < V - 1; i++) v[i] = lane == 0 && (unsigned)i < off ? kNegInf : v[i];
+            }
+            if (step == steps - 1 && keep < V) {
+#pragma unroll
+                for (int q = 0; q < U; q++) {
+                    const bool last = (step * U + q) * 64 + lane == n_units - 1;
+#pragma unroll
+                    for (int i = 1; i < V; i++) v[q * V + i] = last && (unsigned)i >= keep ? kNegInf : v[q * V + i];
                 }
             }
 #pragma unroll
@@ -344,11 +389,14 @@ __global__ __launch_bounds__(256, 8) void logprob_stream_kernel(LogprobArgs a)
             }
             s += es;
             u += eu;
-            if (a.top) {
+            if (TOP) {
                 if (step == 0) best.least = reached_by(top, a.top);
                 if (__ballot(top >= best.least)) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) best.offer(v[e], j0 - off + ((step * U + e / V) * 64 + lane) * V + e % V, a.top, lane);
+                    const auto label = [&](int e) { return j0 - off + ((step * U + e / V) * 64 + lane) * V + e % V; };
+                    best.offer(v, a.top, lane, label, [&](int e) {
+                        const unsigned l = label(e);   // modulo 2^32: one before the piece is far behind it
+                        return l - j0 < j1 - j0 ? to_f32(x[l]) : kNegInf;
+                    });
                 }
             }
 #pragma unroll
@@ -371,18 +419,15 @@ __global__ __launch_bounds__(256, 8) void logprob_stream_kernel(LogprobArgs a)
             } else
                 a.part[work] = r;
         }
-        if (!a.top) continue;
-        if (best.n > 64) best.shrink(a.top, lane);
-        __builtin_amdgcn_wave_barrier();
+        if (!TOP) continue;
+        const unsigned long long key = best.finish(a.top, lane);
         if (a.pieces == 1)
-            logprob_write_list(a, row, r, log_s, best.list, best.n, lane);
+            logprob_write_list(a, row, r, log_s, key, best.n, lane);
         else {
-            const unsigned long long key = lane < best.n ? best.list[lane] : 0;
             const int place = key_place(key, best.n);
             if (lane < best.n && place < a.top) a.part_top[work * a.top + place] = key;
             if (lane >= best.n && lane < a.top) a.part_top[work * a.top + lane] = 0;
         }
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -423,7 +468,8 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
         if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
         unsigned long long border;
-        int n = keep_best(k, a.top, lane, s_list, border);
+        const auto put = [&](int at, unsigned long long key) { s_list[at] = key; };
+        int n = keep_best(k, a.top, border, put);
         for (unsigned long long k0 = 1024; k0 < all; k0 += 960) {   // more pieces: with the best so far in the first place
             __builtin_amdgcn_wave_barrier();
             k[0] = lane < n ? s_list[lane] : 0;
@@ -433,10 +479,10 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
                 k[i] = at < all ? keys[at] : 0;
             }
             __builtin_amdgcn_wave_barrier();
-            n = keep_best(k, a.top, lane, s_list, border);
+            n = keep_best(k, a.top, border, put);
         }
         __builtin_amdgcn_wave_barrier();
-        logprob_write_list(a, row, r, log_s, s_list, n, lane);
+        logprob_write_list(a, row, r, log_s, lane < n ? s_list[lane] : 0, n, lane);
         __builtin_amdgcn_wave_barrier();
     }
 }

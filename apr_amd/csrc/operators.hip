@@ -91,7 +91,9 @@ void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPla
     // few waves: one in a workgroup, so that they spread over the CUs
     const unsigned long long works = a.n * a.pieces;
     const unsigned waves = works < 4ull * v.n_cus ? 1 : 4;
-    hipLaunchKernelGGL(logprob_stream_kernel<T>, dim3((unsigned)std::min<unsigned long long>((works + waves - 1) / waves, kMostBlocks)), dim3(64 * waves), 0, v.stream, a);
+    const dim3 grid((unsigned)std::min<unsigned long long>((works + waves - 1) / waves, kMostBlocks)), block(64 * waves);
+    if (a.top) hipLaunchKernelGGL((logprob_stream_kernel<T, true>), grid, block, 0, v.stream, a);
+    else hipLaunchKernelGGL((logprob_stream_kernel<T, false>), grid, block, 0, v.stream, a);
 }
 
 // The smallest group of lanes that holds a row's 16-byte units in registers

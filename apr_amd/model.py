@@ -112,11 +112,17 @@ def _as_u8(buf) -> np.ndarray:
 
 
 _I8 = 3                              # int8, beside the _capi.F32 / F16 / BF16 of the C ABI
-_ELEMENT_TYPES = {"torch.float32": _capi.F32, "torch.float16": _capi.F16, "torch.bfloat16": _capi.BF16, "torch.int8": _I8}
+_types: dict = {}                    # torch dtype -> element type; filled when the first tensor comes (torch is imported then)
 
 
 def _element_type(t) -> int:
-    return _ELEMENT_TYPES.get(str(t.dtype), -1)
+    if not _types:
+        import torch
+        _types.update({torch.float32: _capi.F32, torch.float16: _capi.F16, torch.bfloat16: _capi.BF16, torch.int8: _I8, torch.int32: _I32})
+    return _types.get(t.dtype, -1)
+
+
+_I32 = 4
 
 
 def torch_stream(engine: "Engine"):
@@ -347,21 +353,31 @@ class Engine:
     def _matrix(self, name: str, a, rows: int, cols: int, ld: Optional[int], dtype: Optional[int] = None, types=(0, 1, 2)):
         """(address, row stride, element type) of a [rows, cols] operand.  A tensor speaks for itself and is checked; for an
         address the caller gives ``ld`` (default: cols) and ``dtype``."""
-        if isinstance(a, int):
-            return a, cols if ld is None else ld, types[0] if dtype is None else dtype
+        try:    # the good case first: a call of the smallest size is bound by this code
+            code = _types[a.dtype]
+            if code in types and a.dim() == 2 and a.get_device() == self.device and (dtype is None or code == dtype):
+                r, c = a.shape
+                step, one = a.stride()
+                if r >= rows and c >= cols and one == 1 and rows > 1 and (ld is None or ld == step):
+                    return a.data_ptr(), step, code
+        except (AttributeError, KeyError):
+            if isinstance(a, int):
+                return a, cols if ld is None else ld, types[0] if dtype is None else dtype
         if not hasattr(a, "data_ptr"):
             raise TypeError(f"{name}: a torch tensor on the engine's GPU or a device address, not {type(a).__name__}")
         code = _element_type(a)
         if code not in types or (dtype is not None and code != dtype):
             raise ValueError(f"{name}: {a.dtype} is not the element type this operand has")
-        if not a.is_cuda or a.device.index != self.device:
+        if a.get_device() != self.device:
             raise ValueError(f"{name} is on {a.device}, the engine on GPU {self.device}")
-        if a.dim() == 2:
-            if a.shape[0] < rows or a.shape[1] < cols:
-                raise ValueError(f"{name}: {tuple(a.shape)} does not hold {rows} x {cols}")
-            if cols > 1 and a.stride(1) != 1:
+        shape = a.shape
+        if len(shape) == 2:
+            if shape[0] < rows or shape[1] < cols:
+                raise ValueError(f"{name}: {tuple(shape)} does not hold {rows} x {cols}")
+            step = a.stride()
+            if cols > 1 and step[1] != 1:
                 raise ValueError(f"{name}: the elements of a row have to be contiguous")
-            own = a.stride(0) if rows > 1 else max(a.shape[1], cols)
+            own = step[0] if rows > 1 else max(shape[1], cols)
             if ld is not None and ld != own and rows > 1:
                 raise ValueError(f"{name}: its rows are {own} elements apart, not {ld}")
             return a.data_ptr(), own, code
@@ -370,17 +386,21 @@ class Engine:
             raise ValueError(f"{name}: {tuple(a.shape)} does not hold {rows} x {cols} at a row stride of {ld}")
         return a.data_ptr(), ld, code
 
-    def _vector(self, name: str, a, count: int, kind: str) -> int:
-        """address of `count` contiguous float32 / int32 values (0 for None)"""
+    def _vector(self, name: str, a, count: int, kind: int = _capi.F32) -> int:
+        """address of `count` contiguous float32 (int32: kind _I32) values (0 for None)"""
         if a is None:
             return 0
-        if isinstance(a, int):
-            return a
+        try:    # the good case first: a call of the smallest size is bound by this code
+            if _types[a.dtype] == kind and a.is_contiguous() and a.numel() >= count and a.get_device() == self.device:
+                return a.data_ptr()
+        except (AttributeError, KeyError):
+            if isinstance(a, int):
+                return a
         if not hasattr(a, "data_ptr"):
             raise TypeError(f"{name}: a torch tensor on the engine's GPU or a device address, not {type(a).__name__}")
-        if str(a.dtype) != "torch." + kind or not a.is_contiguous() or a.numel() < count:
-            raise ValueError(f"{name}: {count} contiguous {kind} values are needed, not {tuple(a.shape)} of {a.dtype}")
-        if not a.is_cuda or a.device.index != self.device:
+        if _element_type(a) != kind or not a.is_contiguous() or a.numel() < count:
+            raise ValueError(f"{name}: {count} contiguous {'int32' if kind == _I32 else 'float32'} values are needed, not {tuple(a.shape)} of {a.dtype}")
+        if a.get_device() != self.device:
             raise ValueError(f"{name} is on {a.device}, the engine on GPU {self.device}")
         return a.data_ptr()
 
@@ -393,13 +413,20 @@ class Engine:
                               ld: Optional[int] = None, dtype: Optional[int] = None, work_bytes: Optional[int] = None) -> None:
         """apr_label_logprobs_device: log probability of each row's label, entropy, the `top` best labels with theirs."""
         x, ld, code = self._matrix("d_logits", d_logits, n, n_labels, ld, dtype)
-        if work_bytes is None:
-            work_bytes = d_work.numel() * d_work.element_size() if hasattr(d_work, "numel") else 0
+        work = d_work
+        if d_work is None or isinstance(d_work, int):
+            work, work_bytes = work or 0, work_bytes or 0
+        else:
+            if not d_work.is_contiguous() or d_work.get_device() != self.device:
+                raise ValueError(f"d_work is contiguous memory on GPU {self.device}")
+            work, size = d_work.data_ptr(), d_work.numel() * d_work.element_size()
+            if work_bytes is None or work_bytes > size:
+                work_bytes = size
         self._chk(self._lib.apr_label_logprobs_device(
-            self._h, code, x, n, n_labels, ld, scale, self._vector("d_target", d_target, n, "int32"), top,
-            self._vector("d_logprob", d_logprob, n, "float32"), self._vector("d_entropy", d_entropy, n, "float32"),
-            self._vector("d_stat", d_stat, 2 * n, "float32"), self._vector("d_top_label", d_top_label, n * top, "int32"),
-            self._vector("d_top_logprob", d_top_logprob, n * top, "float32"), _addr(d_work), work_bytes))
+            self._h, code, x, n, n_labels, ld, scale, self._vector("d_target", d_target, n, _I32), top,
+            self._vector("d_logprob", d_logprob, n), self._vector("d_entropy", d_entropy, n),
+            self._vector("d_stat", d_stat, 2 * n), self._vector("d_top_label", d_top_label, n * top, _I32),
+            self._vector("d_top_logprob", d_top_logprob, n * top), work, work_bytes))
 
     def label_logprobs_backward_device(self, d_logits, n: int, n_labels: int, d_target, d_stat, d_grad, d_g_logprob=None,
                                        d_entropy=None, d_g_entropy=None, scale: float = 1.0, ld: Optional[int] = None,
@@ -408,16 +435,16 @@ class Engine:
         x, ld, code = self._matrix("d_logits", d_logits, n, n_labels, ld, dtype)
         grad, ld_grad, _ = self._matrix("d_grad", d_grad, n, n_labels, ld_grad, code)
         self._chk(self._lib.apr_label_logprobs_backward_device(
-            self._h, code, x, n, n_labels, ld, scale, self._vector("d_target", d_target, n, "int32"),
-            self._vector("d_stat", d_stat, 2 * n, "float32"), self._vector("d_entropy", d_entropy, n, "float32"),
-            self._vector("d_g_logprob", d_g_logprob, n, "float32"), self._vector("d_g_entropy", d_g_entropy, n, "float32"), grad, ld_grad))
+            self._h, code, x, n, n_labels, ld, scale, self._vector("d_target", d_target, n, _I32),
+            self._vector("d_stat", d_stat, 2 * n), self._vector("d_entropy", d_entropy, n),
+            self._vector("d_g_logprob", d_g_logprob, n), self._vector("d_g_entropy", d_g_entropy, n), grad, ld_grad))
 
     def quantize_rows_device(self, d_x, n: int, k: int, d_q, d_scale, ld: Optional[int] = None, ld_q: Optional[int] = None,
                              dtype: Optional[int] = None) -> None:
         """apr_quantize_rows_device: rows as int8 with one float32 scale each."""
         x, ld, code = self._matrix("d_x", d_x, n, k, ld, dtype)
         q, ld_q, _ = self._matrix("d_q", d_q, n, k, ld_q, None, (_I8,))
-        self._chk(self._lib.apr_quantize_rows_device(self._h, code, x, n, k, ld, q, ld_q, self._vector("d_scale", d_scale, n, "float32")))
+        self._chk(self._lib.apr_quantize_rows_device(self._h, code, x, n, k, ld, q, ld_q, self._vector("d_scale", d_scale, n)))
 
     def linear_i8_device(self, d_x, d_x_scale, d_w, d_w_scale, m: int, n: int, k: int, d_out, d_bias=None, ld_x: Optional[int] = None,
                          ld_w: Optional[int] = None, ld_out: Optional[int] = None, dtype: Optional[int] = None) -> None:
@@ -426,8 +453,8 @@ class Engine:
         w, ld_w, _ = self._matrix("d_w", d_w, n, k, ld_w, None, (_I8,))
         out, ld_out, code = self._matrix("d_out", d_out, m, n, ld_out, dtype)
         self._chk(self._lib.apr_linear_i8_device(
-            self._h, x, ld_x, self._vector("d_x_scale", d_x_scale, m, "float32"), w, ld_w, self._vector("d_w_scale", d_w_scale, n, "float32"),
-            self._vector("d_bias", d_bias, n, "float32"), m, n, k, code, out, ld_out))
+            self._h, x, ld_x, self._vector("d_x_scale", d_x_scale, m), w, ld_w, self._vector("d_w_scale", d_w_scale, n),
+            self._vector("d_bias", d_bias, n), m, n, k, code, out, ld_out))
 
     @property
     def num_features(self) -> int:

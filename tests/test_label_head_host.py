@@ -86,13 +86,13 @@ def test_python_side_refuses_host_and_foreign_tensors():
     with pytest.raises(ValueError, match="element type"):
         e._matrix("d_q", torch.zeros(2, 3), 2, 3, None, None, (model._I8,))
     with pytest.raises(TypeError):
-        e._vector("d_scale", np.zeros(2, np.float32), 2, "float32")
+        e._vector("d_scale", np.zeros(2, np.float32), 2)
     with pytest.raises(ValueError, match="float32"):
-        e._vector("d_scale", torch.zeros(2, dtype=torch.int32), 2, "float32")
+        e._vector("d_scale", torch.zeros(2, dtype=torch.int32), 2)
     with pytest.raises(ValueError, match="on cpu"):
-        e._vector("d_scale", torch.zeros(2), 2, "float32")
+        e._vector("d_scale", torch.zeros(2), 2)
     assert e._matrix("d_x", 4096, 2, 3, None) == (4096, 3, _capi.F32) and e._matrix("d_x", 4096, 2, 3, 8, _capi.BF16) == (4096, 8, _capi.BF16)
-    assert e._vector("d_scale", None, 2, "float32") == 0
+    assert e._vector("d_scale", None, 2) == 0
 
 
 @pytest.mark.parametrize("scale", [1.0, 0.37])

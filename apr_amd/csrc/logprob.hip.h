@@ -442,6 +442,12 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
         unsigned long long k[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) k[i] = 64u * i + lane < all ? keys[64 * i + lane] : 0;
+        unsigned long long sample = 0;
+        if (a.top && a.pieces < 64) {
+            const unsigned each = 64 / a.pieces, p = lane / each, j = lane - p * each;
+            if (p < a.pieces && j < (unsigned)a.top) sample = keys[(unsigned long long)p * a.top + j];
+        } else if (a.top)
+            for (unsigned p = lane; p < a.pieces; p += 64) sample = max(sample, keys[(unsigned long long)p * a.top]);
         const LogprobPart *part = a.part + row * a.pieces;
         const int t = a.target ? a.target[row] : -1;
         const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
@@ -467,9 +473,28 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
         const float log_s = log_of_sum(r.s);
         if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
+        // A score that `top` of 64 of the keys reach, each piece's best or as many of each as make 64, bounds the ones that matter: about
+        // as many as are wanted.  keep_best, which counts all keys 16 times, is for what is left over that.
         unsigned long long border;
         const auto put = [&](int at, unsigned long long key) { s_list[at] = key; };
-        int n = keep_best(k, a.top, border, put);
+        const float least = reached_by(sample ? key_score(sample) : kNegInf, a.top);
+        const unsigned long long reach = score_key(least, 0) >> 32 << 32;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            if (k[i] < reach) k[i] = 0;
+            n += __builtin_popcountll(__ballot(k[i] != 0));
+        }
+        if (n <= 64) {
+            n = 0;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const unsigned long long mask = __ballot(k[i] != 0);
+                if (k[i]) put(n + below(mask), k[i]);
+                n += __builtin_popcountll(mask);
+            }
+        } else
+            n = keep_best(k, a.top, border, put);
         for (unsigned long long k0 = 1024; k0 < all; k0 += 960) {   // more pieces: with the best so far in the first place
             __builtin_amdgcn_wave_barrier();
             k[0] = lane < n ? s_list[lane] : 0;
@@ -493,7 +518,10 @@ struct LogprobPlan {
     unsigned pieces, piece_len;
     size_t work;   // bytes
 };
-constexpr size_t kWavesWanted = 4096, kLeastPiece = 4096;
+// Waves that fill the chip in one round (the form with alternatives has places for 5120: 2000 rows in two pieces take 116 us, in three
+// pieces, a round and a bit, 133).  A piece is a step at least, and the pieces' alternatives are as many as the join holds at once (one
+// row of 131071, 20 alternatives: 16 us in 33 pieces, 18 in 65, whose lists it takes in two goes, and 22 in 17).
+constexpr size_t kWavesWanted = 3200, kStep = 1024, kJoined = 1024;
 inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
 {
     LogprobPlan p = {0, 1, (unsigned)c, 0};
@@ -501,8 +529,9 @@ inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
         p.each = (int)((c + 63) / 64);
         return p;
     }
-    // pieces while the rows alone are too few waves for the chip
-    const size_t pieces = std::min((kWavesWanted + n - 1) / std::max<size_t>(n, 1), (c + kLeastPiece - 1) / kLeastPiece);
+    // pieces while the rows alone are too few waves
+    size_t pieces = std::min((kWavesWanted + n - 1) / std::max<size_t>(n, 1), (c + kStep - 1) / kStep);
+    if (top > 0) pieces = std::min(pieces, kJoined / (size_t)top);
     p.piece_len = (unsigned)(((c + pieces - 1) / pieces + 7) / 8 * 8);
     p.pieces = (unsigned)((c + p.piece_len - 1) / p.piece_len);
     if (p.pieces > 1) p.work = n * p.pieces * (size_t)top * 8 + (n * p.pieces * sizeof(LogprobPart) + 15) / 16 * 16;

@@ -211,9 +211,10 @@ int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_l
     LogprobGradArgs a;
     a.x = d_logits; a.grad = d_grad; a.n = n; a.ld = ld; a.ld_grad = ld_grad; a.n_labels = (unsigned)n_labels; a.scale = (float)scale;
     a.target = d_target; a.stat = d_stat; a.entropy = d_entropy; a.g_logprob = d_g_logprob; a.g_entropy = d_g_entropy;
-    // pieces of 512 units or more, while the rows alone are too few waves for the chip
+    // pieces of 512 units or more, while the rows alone are too few waves
+    constexpr size_t kGradWaves = 8192;
     const size_t units = std::max<size_t>(n_labels * element_size(dtype) / 16, 1);
-    const size_t pieces = std::max<size_t>(1, std::min((2 * kWavesWanted + n - 1) / n, units / 512));
+    const size_t pieces = std::max<size_t>(1, std::min((kGradWaves + n - 1) / n, units / 512));
     a.piece_units = (unsigned)((units + pieces - 1) / pieces);
     a.pieces = (unsigned)((units + a.piece_units - 1) / a.piece_units);
     return on_engine(e, me, [&](const EngineView &v) {

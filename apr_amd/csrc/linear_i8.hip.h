@@ -22,6 +22,23 @@ struct LinearI8Args {
     unsigned m, n, k;
 };
 
+// 16 bytes of a row from k on, 0 from `end` on.  WHOLE: the rows are 16-byte aligned, and the unit that k ends in is read whole (it lies in
+// the row's stride, and inside the allocation, as its first byte is); otherwise a unit begins at any byte, and the one that k ends in is
+// read byte by byte.
+template <bool WHOLE>
+__device__ __forceinline__ i32x4 linear_unit(const int8_t *row, unsigned k, unsigned end)
+{
+    i32x4 v = {0, 0, 0, 0};
+    if (k >= end) return v;
+    if (WHOLE) return *(const i32x4 *)(row + k);
+    if (k + 16u <= end) {
+        __builtin_memcpy(&v, row + k, 16);
+        return v;
+    }
+    for (unsigned c = 0; k + c < end; c++) v[c >> 2] |= (int)(uint8_t)row[k + c] << (8 * (c & 3));
+    return v;
+}
+
 // ---- tiled kernel: operands 16 bytes at a time, straight from memory to LDS ----
 //
 // A stage is BK bytes of k of every row of the tile, [row][BK / 16 units of 16 bytes]; unit c of row r lies at place
@@ -57,7 +74,8 @@ __device__ __forceinline__ void linear_tile(unsigned block, unsigned tiles_m, un
     tm = g * G + in - tn * rows;
 }
 
-template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN>
+// DMA false: rows that are not 16-byte aligned.  The stages come through registers, a step ahead, and are written to the same places.
+template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN, bool DMA>
 __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI8Args a, unsigned tiles_m, unsigned tiles_n)
 {
     constexpr int WAVES = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32, KS = BK / 32, UNITS = BK / 16, RPD = 64 / UNITS;
@@ -91,7 +109,24 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
     const unsigned full = a.k / BK, steps = (a.k + BK - 1) / BK;
     unsigned k_next = 0;   // first k of the next stage to fetch
     int slot_in = 0;
+    static_assert(DMA || NBUF == 2, "one stage is in registers");
+    i32x4 hx[DMA ? 1 : DA], hw[DMA ? 1 : DB];
     auto fetch = [&]() {
+        if (!DMA) {
+            const unsigned k = k_next + 16u * du;
+#pragma unroll
+            for (int i = 0; i < DA; i++) {
+                const unsigned r = (wave * DA + i) * RPD + dr;
+                hx[DMA ? 0 : i] = linear_unit<false>(a.x + (m0 + r) * a.ld_x, k, r < rows_x ? a.k : 0);
+            }
+#pragma unroll
+            for (int i = 0; i < DB; i++) {
+                const unsigned r = (wave * DB + i) * RPD + dr;
+                hw[DMA ? 0 : i] = linear_unit<false>(a.w + (n0 + r) * a.ld_w, k, r < rows_w ? a.k : 0);
+            }
+            k_next += BK;
+            return;
+        }
         if (k_next < a.k) {
             const i32x4 rx = {(int)(unsigned)bx, (int)(unsigned)(bx >> 32), (int)nx, 0x00020000};
             const i32x4 rw = {(int)(unsigned)bw, (int)(unsigned)(bw >> 32), (int)nw, 0x00020000};
@@ -114,6 +149,16 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
         }
         k_next += BK;
         slot_in = slot_in + 1 == NBUF ? 0 : slot_in + 1;
+    };
+
+    auto commit = [&]() {   // what fetch left in registers
+        if (DMA) return;
+        int8_t *to = lds + slot_in * STAGE + lane * 16;
+#pragma unroll
+        for (int i = 0; i < DA; i++) *(i32x4 *)(to + (wave * DA + i) * 1024) = hx[DMA ? 0 : i];
+#pragma unroll
+        for (int i = 0; i < DB; i++) *(i32x4 *)(to + ABYTES + (wave * DB + i) * 1024) = hw[DMA ? 0 : i];
+        slot_in ^= 1;
     };
 
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN), r32 = lane & 31, half = lane >> 5;
@@ -140,6 +185,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
     constexpr int FLY = (NBUF - 2) * (DA + DB);   // loads that may still be on their way when the next stage has to be there
 #pragma unroll
     for (int s = 0; s < NBUF - 1; s++) fetch();
+    commit();
     wait_dma_and_meet<FLY>();
     unsigned stage = 0;
     if (full) read(0, 0, 0);
@@ -150,6 +196,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
         for (int kk = 0; kk < KS; kk++) {
             if (kk + 1 < KS) read((kk + 1) & 1, stage, kk + 1);
             else {
+                commit();
                 wait_dma_and_meet<FLY>();
                 read(0, next, 0);   // past the last whole stage: the tail's, or zeros
             }
@@ -231,70 +278,68 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
     }
 }
 
-// ---- few tiles: every wave takes a part of k for the same 32 x 32 outputs, straight from memory to registers ----
+// ---- few tiles: every wave takes a part of k for the same 16 n and G x 16 m, straight from memory to registers ----
 //
-// Blocks of 128 k go to the W waves in turn; a lane reads the four 16-byte units of its row that the block's four matrix instructions
-// want (they share the row's cache lines).  The waves' partial sums, exact whole numbers, meet in LDS.
-// WHOLE: the rows are 16-byte aligned, and the unit that k ends in is read whole (it lies in the row's stride) and cut in x.
-// Otherwise a unit begins at any byte, and the one that k ends in is read byte by byte.
-template <bool WHOLE>
-__device__ __forceinline__ i32x4 linear_unit(const int8_t *row, unsigned k, unsigned end)
+// Blocks of 256 k go to the W waves in turn.  A load takes 64 neighbouring bytes of 16 rows (the 16 x 16 x 64 instruction's layout: with the
+// 32 x 32 x 32 one a load takes 32 bytes of 32 rows, and the lines of 16 waves do not stay in the L1 until the rest is asked for:
+// 1 x 8192 x 8192 takes 14.0 us against 19.4, 4.8 TB/s of weights, the rate of a copy).  The waves' partial sums, exact whole numbers, meet in LDS.
+template <typename T, int W, int G, bool WHOLE>
+__global__ __launch_bounds__(W * 64) void linear_i8_few_kernel(LinearI8Args a)
 {
-    i32x4 v = {0, 0, 0, 0};
-    if (k >= end) return v;
-    if (WHOLE) return *(const i32x4 *)(row + k);
-    if (k + 16u <= end) {
-        __builtin_memcpy(&v, row + k, 16);
-        return v;
-    }
-    for (unsigned c = 0; k + c < end; c++) v[c >> 2] |= (int)(uint8_t)row[k + c] << (8 * (c & 3));
-    return v;
-}
-
-template <typename T, int W, bool WHOLE>
-__global__ __launch_bounds__(W * 64, 1) void linear_i8_few_kernel(LinearI8Args a)
-{
-    __shared__ int s_part[W][16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
-    const unsigned long long tiles_n = (a.n + 31u) / 32u, tiles = (a.m + 31u) / 32u * tiles_n;
-    const unsigned blocks = (a.k + 127u) / 128u;
+    __shared__ int s_part[W][G * 4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, quarter = lane >> 4;
+    const unsigned long long tiles_n = (a.n + 15u) / 16u, tiles = (a.m + 16u * G - 1u) / (16u * G) * tiles_n;
+    const unsigned blocks = (a.k + 255u) / 256u;
     for (unsigned long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const unsigned m0 = (unsigned)(tile / tiles_n) * 32u, n0 = (unsigned)(tile % tiles_n) * 32u;
-        const unsigned k_x = m0 + r32 < a.m ? a.k : 0, k_w = n0 + r32 < a.n ? a.k : 0;   // a row past the matrix has no units
-        const int8_t *x = a.x + (m0 + r32) * a.ld_x, *w = a.w + (n0 + r32) * a.ld_w;
-        i32x16 acc = {};
-        i32x4 fx[4], fw[4];
+        const unsigned m0 = (unsigned)(tile / tiles_n) * (16u * G), n0 = (unsigned)(tile % tiles_n) * 16u;
+        const unsigned k_w = n0 + r16 < a.n ? a.k : 0;   // a row past the matrix has no units
+        const int8_t *w = a.w + (n0 + r16) * a.ld_w, *x[G];
+        unsigned k_x[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            k_x[g] = m0 + 16 * g + r16 < a.m ? a.k : 0;
+            x[g] = a.x + (m0 + 16 * g + r16) * a.ld_x;
+        }
+        i32x4 acc[G] = {}, fw[4], fx[G][4];
         auto load = [&](unsigned b) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                fw[u] = linear_unit<WHOLE>(w, b * 128u + 32u * u + 16u * half, k_w);
-                fx[u] = linear_unit<WHOLE>(x, b * 128u + 32u * u + 16u * half, k_x);
+                const unsigned k = b * 256u + 64u * u + 16u * quarter;
+                fw[u] = linear_unit<WHOLE>(w, k, k_w);
+#pragma unroll
+                for (int g = 0; g < G; g++) fx[g][u] = linear_unit<WHOLE>(x[g], k, k_x[g]);
             }
         };
         load(wave);
         for (unsigned b = wave; b < blocks; b += W) {
-            if (WHOLE && b * 128u + 128u > a.k) {
+            if (WHOLE && b * 256u + 256u > a.k) {
 #pragma unroll
                 for (int u = 0; u < 4; u++)
 #pragma unroll
                     for (int d = 0; d < 4; d++) {
-                        const int keep = (int)a.k - (int)(b * 128u + 32u * u + 16u * half) - 4 * d;
-                        fx[u][d] &= keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+                        const int keep = (int)a.k - (int)(b * 256u + 64u * u + 16u * quarter) - 4 * d;
+                        const int mask = keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+#pragma unroll
+                        for (int g = 0; g < G; g++) fx[g][u][d] &= mask;
                     }
             }
 #pragma unroll
-            for (int u = 0; u < 4; u++) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[u], fw[u], acc, 0, 0, 0);
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int g = 0; g < G; g++) acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fx[g][u], fw[u], acc[g], 0, 0, 0);
             load(b + W);
         }
         __syncthreads();   // the last tile's sums are read
 #pragma unroll
-        for (int e = 0; e < 16; e++) s_part[wave][e][lane] = acc[e];
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s_part[wave][4 * g + e][lane] = acc[g][e];
         __syncthreads();
-        for (int e = wave; e < 16; e += W) {
+        for (int e = wave; e < 4 * G; e += W) {
             int sum = 0;
 #pragma unroll
             for (int v = 0; v < W; v++) sum += s_part[v][e][lane];
-            const unsigned m = m0 + 8 * (e >> 2) + 4 * half + (e & 3), n = n0 + r32;
+            const unsigned m = m0 + 16 * (e >> 2) + 4 * quarter + (e & 3), n = n0 + r16;
             if (m < a.m && n < a.n) ((T *)a.out)[m * a.ld_out + n] = from_f32<T>((float)sum * a.x_scale[m] * a.w_scale[n] + (a.bias ? a.bias[n] : 0.0f));
         }
     }
@@ -305,26 +350,30 @@ __global__ __launch_bounds__(W * 64, 1) void linear_i8_few_kernel(LinearI8Args a
 // Microseconds of a variant: t0 for each tile that a CU walks one after the other, and a step of 128 k takes `alone` (its latency,
 // shared by the `beside` tiles that fit a CU together) or `full` for each tile (its throughput), whichever is longer.  Measured with
 // one to eight rounds of tiles, bf16 out; 1024 x 8192 x 8192: 98 / 73 / 121 / 103 us by 256 x 256, 128 x 128, 64 x 64 with four and with
-// two stages (the rule: 98 / 73 / 126 / 108), 256 x 8192 x 8192: 85 / 50 / 32 / 39 (98 / 50 / 32 / 39), 16384 x 8192 x 8192: 925 / 1113 / 1780 / 1612.
-// The `few` kernel: per 32 x 32 tile of a CU 2.5 us and 1.9 us for each 1024 k: 256 x 527 x 1024 takes 4.4 us against 6.7, 4096 x 527 x 1024 30 against 9.4.
+// two stages (the rule: 98 / 73 / 127 / 105), 256 x 8192 x 8192: 85 / 50 / 32 / 39 (98 / 50 / 34 / 39), 16384 x 8192 x 8192: 925 / 1113 / 1780 / 1612.
+// The few kernel: 2.3 us and, for each tile of a CU, 0.8 ns a k (16 m) or 1.4 ns a k (32 m): 256 x 527 x 1024 takes 5.1 us against 6.7 by
+// 64 x 64 tiles, 64 x 2000 x 4096 8.7; 4096 x 527 x 1024 would take 30 against 9.4.
 struct LinearCost {
     int tile, beside;
     float t0, alone, full;
 };
-constexpr LinearCost kLinearCost[4] = {{256, 1, 5.0f, 1.45f, 1.72f}, {128, 2, 3.6f, 0.73f, 0.54f}, {64, 2, 2.5f, 0.30f, 0.24f}, {64, 5, 2.5f, 0.57f, 0.20f}};
+constexpr LinearCost kLinearCost[4] = {{256, 1, 5.0f, 1.45f, 1.72f}, {128, 2, 3.6f, 0.73f, 0.54f}, {64, 2, 3.5f, 0.29f, 0.24f}, {64, 5, 2.5f, 0.57f, 0.20f}};
 enum { kLinear256, kLinear128, kLinear64Deep, kLinear64, kLinearFew };
 
-inline int linear_variant(unsigned m, unsigned n, unsigned k, int n_cus)
+// whole: the rows are 16-byte aligned; otherwise there are 128 x 128 tiles, whose steps then take about twice as long, and the few kernel,
+// which takes four times as long
+inline int linear_variant(unsigned m, unsigned n, unsigned k, bool whole, int n_cus)
 {
     const float steps = (float)((k + 127) / 128), cus = (float)n_cus;
-    const float few_tiles = (float)((m + 31) / 32) * (float)((n + 31) / 32);
-    float best = ceilf(few_tiles / cus) * (2.5f + 1.9e-3f * (float)k);
+    const float few_tiles = (float)(m <= 16 ? 1 : (m + 31) / 32) * (float)((n + 15) / 16);
+    float best = 2.3f + ceilf(few_tiles / cus) * (m <= 16 ? 0.8e-3f : 1.4e-3f) * (float)k * (whole ? 1.0f : 4.0f);
     int variant = kLinearFew;
     for (int v = 0; v < 4; v++) {
+        if (!whole && v != kLinear128) continue;
         const LinearCost &c = kLinearCost[v];
         const float tiles = (float)((m + c.tile - 1) / c.tile) * (float)((n + c.tile - 1) / c.tile);
         const float per_cu = ceilf(tiles / cus), rounds = ceilf(per_cu / (float)c.beside);
-        const float us = c.t0 * rounds + steps * fmaxf(c.alone * rounds, c.full * per_cu);
+        const float us = c.t0 * rounds + steps * fmaxf(c.alone * rounds, c.full * per_cu) * (whole ? 1.0f : 2.0f);
         if (us < best) { best = us; variant = v; }
     }
     return variant;

@@ -116,11 +116,11 @@ void launch_rowquant(const EngineView &v, const RowQuantArgs &a)
 }
 
 // Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.
-template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN>
+template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN, bool DMA = true>
 void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
 {
     constexpr int bytes = (BM + BN) * BK * NBUF;
-    const auto kernel = linear_i8_tile_kernel<T, BM, BN, BK, NBUF, WM, WN>;
+    const auto kernel = linear_i8_tile_kernel<T, BM, BN, BK, NBUF, WM, WN, DMA>;
     static std::atomic<uint64_t> allowed{0};
     const uint64_t bit = 1ull << (v.device & 63);
     if (bytes > 65536 && !(allowed.load(std::memory_order_relaxed) & bit)) {
@@ -134,14 +134,18 @@ void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
 template <typename T>
 void launch_linear(const EngineView &v, const LinearI8Args &a)
 {
-    const unsigned long long few = (unsigned long long)((a.m + 31) / 32) * ((a.n + 31) / 32);
+    const unsigned long long few = (unsigned long long)(a.m <= 16 ? 1 : (a.m + 31) / 32) * ((a.n + 15) / 16);
     const dim3 few_grid((unsigned)std::min<unsigned long long>(few, kMostBlocks));
     const bool whole = aligned(a.x, 16) && aligned(a.w, 16) && a.ld_x % 16 == 0 && a.ld_w % 16 == 0;
-    int variant = linear_variant(a.m, a.n, a.k, v.n_cus);
+    int variant = linear_variant(a.m, a.n, a.k, whole, v.n_cus);
     // the tiles address their rows with 32 bits, and a grid has less than 2^32 threads
-    if (a.ld_x > (1u << 22) || a.ld_w > (1u << 22) || few > (1ull << 24)) variant = kLinearFew;
-    if (!whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 4, false>), few_grid, dim3(256), 0, v.stream, a);
-    else if (variant == kLinearFew) hipLaunchKernelGGL((linear_i8_few_kernel<T, 16, true>), few_grid, dim3(1024), 0, v.stream, a);
+    if (a.ld_x > (1u << 22) || a.ld_w > (1u << 22) || few > (1ull << 25)) variant = kLinearFew;
+    if (variant == kLinearFew) {
+        if (a.m <= 16 && whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 1, true>), few_grid, dim3(512), 0, v.stream, a);
+        else if (a.m <= 16) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 1, false>), few_grid, dim3(512), 0, v.stream, a);
+        else if (whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 2, true>), few_grid, dim3(512), 0, v.stream, a);
+        else hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 2, false>), few_grid, dim3(512), 0, v.stream, a);
+    } else if (!whole) launch_linear_tiles<T, 128, 128, 128, 2, 2, 2, false>(v, a);
     else if (variant == kLinear256) launch_linear_tiles<T, 256, 256, 128, 2, 2, 4>(v, a);
     else if (variant == kLinear128) launch_linear_tiles<T, 128, 128, 128, 2, 2, 2>(v, a);
     else if (variant == kLinear64Deep) launch_linear_tiles<T, 64, 64, 128, 4, 2, 2>(v, a);

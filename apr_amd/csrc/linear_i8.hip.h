@@ -41,10 +41,16 @@ __device__ __forceinline__ i32x4 linear_unit(const int8_t *row, unsigned k, unsi
 
 // ---- tiled kernel: operands 16 bytes at a time, straight from memory to LDS ----
 //
-// A stage is BK bytes of k of every row of the tile, [row][BK / 16 units of 16 bytes]; unit c of row r lies at place
-// c ^ swizzle(r), so that the eight lanes that an LDS read serves together hit all banks once (rows are 64 or 128 bytes, which
-// alone would put the same unit of all rows on the same banks).  A DMA instruction fills 1 KiB of LDS lane by lane; the swizzle
-// is which unit each lane asks for.  Rows past the matrix and units past k are out of the buffer's range, which reads as 0.
+// A stage is 128 bytes of k of every row of the tile, eight units of 16 bytes; unit c of row r lies at place c ^ ((r >> 1) & 7).  An LDS
+// read of 16 bytes a lane serves 16 lanes at a time, which hit all 64 banks once if their places differ modulo 256 bytes: the
+// hardware's sixteen (lanes 0-3, 12-15, 20-23, 24-27 and so on) are eight even and eight odd rows whose r >> 1 differ modulo 8.
+// (With r & 7 they pair up: 104 million cycles of bank conflicts in a product of 16384 x 8192 x 8192 instead of 3, though not more time.)
+// A DMA instruction fills 1 KiB of LDS, eight rows, lane by lane; the swizzle is which unit each lane asks for.  Rows past the matrix
+// and units past k are out of the buffer's range, which reads as 0.
+//
+// What bounds 256 x 256 tiles: the chip's power.  16384 x 8192 x 8192 takes 0.92-0.95 ms (2.3-2.4 POPS) at 1.8 GHz, where the matrix units work
+// 62 % of the cycles; matrix instructions alone, without loads, take 0.69 ms, since random operands bring the clock down (from
+// registers 3.1-3.5 POPS, and 4.6 on zeros), and with the LDS reads 0.78.
 // LDS-DMA: 64 lanes x 16 B from a buffer to 1 KiB of LDS at byte address lds (wave-uniform).  The caller waits on vmcnt.
 __device__ __forceinline__ void linear_dma(i32x4 rs, unsigned voff, unsigned lds)
 {
@@ -74,8 +80,10 @@ __device__ __forceinline__ void linear_tile(unsigned block, unsigned tiles_m, un
     tm = g * G + in - tn * rows;
 }
 
+// EVERY: a DMA instruction in front of every EVERY-th matrix instruction, so that the 64 KiB of a stage do not queue up before the step's
+// first product (128 x 128 tiles: 2-3 % less time, 256 x 256: 1 %); 0: all at the top (64 x 64 tiles have too few instructions a step).
 // DMA false: rows that are not 16-byte aligned.  The stages come through registers, a step ahead, and are written to the same places.
-template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN, bool DMA>
+template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN, bool DMA, int EVERY>
 __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI8Args a, unsigned tiles_m, unsigned tiles_n)
 {
     constexpr int WAVES = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32, KS = BK / 32, UNITS = BK / 16, RPD = 64 / UNITS;
@@ -95,62 +103,59 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
     // the base along k and not the range
     const unsigned nx = (rows_x - 1) * ld_x + k16, nw = (rows_w - 1) * ld_w + k16;
 
-    // this lane's row and unit of a DMA instruction
+    // this lane's row of a DMA instruction's eight, and its unit: the rows of every other instruction are 8 to 15 modulo 16
+    static_assert(BK == 128 && DA % 2 == 0 && DB % 2 == 0, "units and their places");
     const int dr = lane / UNITS, dp = lane % UNITS;
-    constexpr int SH = UNITS == 8 ? 0 : 1;
+    const int du[2] = {dp ^ (dr >> 1), dp ^ (dr >> 1) ^ 4};
     unsigned vx[DA], vw[DB];
-    const int du = dp ^ ((dr >> SH) & (UNITS - 1));   // RPD is a multiple of the swizzle's period
 #pragma unroll
-    for (int i = 0; i < DA; i++) vx[i] = (unsigned)((wave * DA + i) * RPD + dr) * ld_x + 16u * du;
+    for (int i = 0; i < DA; i++) vx[i] = (unsigned)((wave * DA + i) * RPD + dr) * ld_x + 16u * du[i & 1];
 #pragma unroll
-    for (int i = 0; i < DB; i++) vw[i] = (unsigned)((wave * DB + i) * RPD + dr) * ld_w + 16u * du;
+    for (int i = 0; i < DB; i++) vw[i] = (unsigned)((wave * DB + i) * RPD + dr) * ld_w + 16u * du[i & 1];
     const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) int8_t *)lds;
 
     const unsigned full = a.k / BK, steps = (a.k + BK - 1) / BK;
     unsigned k_next = 0;   // first k of the next stage to fetch
     int slot_in = 0;
     static_assert(DMA || NBUF == 2, "one stage is in registers");
-    i32x4 hx[DMA ? 1 : DA], hw[DMA ? 1 : DB];
+    static_assert(EVERY * (DA + DB - 1) < (KS - 1) * FM * FN || EVERY == 0, "all of a stage is asked for before the waves meet");
+    i32x4 hx[DMA ? 1 : DA], hw[DMA ? 1 : DB], rx, rw;
+    bool past[2];
+    unsigned to;
+    auto piece = [&](int i) {   // one DMA instruction of the stage that fetch has begun
+        if (i < DA) linear_dma(rx, past[i & 1] ? 0xFFFFFFF0u : vx[i], to + (wave * DA + i) * 1024);
+        else linear_dma(rw, past[i & 1] ? 0xFFFFFFF0u : vw[i - DA], to + ABYTES + (wave * DB + i - DA) * 1024);
+    };
     auto fetch = [&]() {
         if (!DMA) {
-            const unsigned k = k_next + 16u * du;
 #pragma unroll
             for (int i = 0; i < DA; i++) {
                 const unsigned r = (wave * DA + i) * RPD + dr;
-                hx[DMA ? 0 : i] = linear_unit<false>(a.x + (m0 + r) * a.ld_x, k, r < rows_x ? a.k : 0);
+                hx[DMA ? 0 : i] = linear_unit<false>(a.x + (m0 + r) * a.ld_x, k_next + 16u * du[i & 1], r < rows_x ? a.k : 0);
             }
 #pragma unroll
             for (int i = 0; i < DB; i++) {
                 const unsigned r = (wave * DB + i) * RPD + dr;
-                hw[DMA ? 0 : i] = linear_unit<false>(a.w + (n0 + r) * a.ld_w, k, r < rows_w ? a.k : 0);
+                hw[DMA ? 0 : i] = linear_unit<false>(a.w + (n0 + r) * a.ld_w, k_next + 16u * du[i & 1], r < rows_w ? a.k : 0);
             }
             k_next += BK;
             return;
         }
-        if (k_next < a.k) {
-            const i32x4 rx = {(int)(unsigned)bx, (int)(unsigned)(bx >> 32), (int)nx, 0x00020000};
-            const i32x4 rw = {(int)(unsigned)bw, (int)(unsigned)(bw >> 32), (int)nw, 0x00020000};
-            const bool tail = k_next + BK > a.k;
-            const bool out = tail && k_next + 16u * du >= a.k;
-            const unsigned base = lds0 + slot_in * STAGE + wave * DA * 1024, basew = lds0 + slot_in * STAGE + ABYTES + wave * DB * 1024;
-#pragma unroll
-            for (int i = 0; i < DA; i++) linear_dma(rx, out ? 0xFFFFFFF0u : vx[i], base + i * 1024);
-#pragma unroll
-            for (int i = 0; i < DB; i++) linear_dma(rw, out ? 0xFFFFFFF0u : vw[i], basew + i * 1024);
-            bx += BK; bw += BK;
-        } else {
-            // an empty stage keeps the count of loads in flight: all lanes out of range
-            const i32x4 r0 = {(int)(unsigned)(unsigned long long)a.x, (int)(unsigned)((unsigned long long)a.x >> 32), 0, 0x00020000};
-            const unsigned base = lds0 + slot_in * STAGE + wave * DA * 1024, basew = lds0 + slot_in * STAGE + ABYTES + wave * DB * 1024;
-#pragma unroll
-            for (int i = 0; i < DA; i++) linear_dma(r0, 0xFFFFFFF0u, base + i * 1024);
-#pragma unroll
-            for (int i = 0; i < DB; i++) linear_dma(r0, 0xFFFFFFF0u, basew + i * 1024);
-        }
+        // past k an empty stage keeps the count of loads in flight: a range of 0
+        const unsigned left = k_next < a.k ? a.k - k_next : 0;
+        rx = {(int)(unsigned)bx, (int)(unsigned)(bx >> 32), left ? (int)nx : 0, 0x00020000};
+        rw = {(int)(unsigned)bw, (int)(unsigned)(bw >> 32), left ? (int)nw : 0, 0x00020000};
+        past[0] = 16u * du[0] >= left;
+        past[1] = 16u * du[1] >= left;
+        to = lds0 + slot_in * STAGE;
+        if (left > BK) { bx += BK; bw += BK; }
         k_next += BK;
         slot_in = slot_in + 1 == NBUF ? 0 : slot_in + 1;
+        if (EVERY == 0) {
+#pragma unroll
+            for (int i = 0; i < DA + DB; i++) piece(i);
+        }
     };
-
     auto commit = [&]() {   // what fetch left in registers
         if (DMA) return;
         int8_t *to = lds + slot_in * STAGE + lane * 16;
@@ -164,7 +169,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN), r32 = lane & 31, half = lane >> 5;
     unsigned pa[KS];   // this lane's place in a row for each k of 32
 #pragma unroll
-    for (int kk = 0; kk < KS; kk++) pa[kk] = (unsigned)(((2 * kk + half) ^ ((r32 >> SH) & (UNITS - 1))) * 16);
+    for (int kk = 0; kk < KS; kk++) pa[kk] = (unsigned)(((2 * kk + half) ^ ((r32 >> 1) & 7)) * 16);
     const int8_t *la = lds + (wm + r32) * BK, *lb = lds + ABYTES + (wn + r32) * BK;
 
     i32x16 acc[FM][FN] = {};
@@ -175,16 +180,33 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
 #pragma unroll
         for (int j = 0; j < FN; j++) fb[set][j] = *(const i32x4 *)(lb + stage + j * 32 * BK + pa[kk]);
     };
-    auto multiply = [&](int set) {
+    // at: matrix instructions of this step before these; every EVERY-th has a DMA instruction in front of it
+    auto multiply = [&](int set, int at) {
 #pragma unroll
         for (int i = 0; i < FM; i++)
 #pragma unroll
-            for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[set][j], fa[set][i], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < FN; j++) {
+                if (EVERY > 0) {
+                    const int q = at + i * FN + j;
+                    if (q >= 0 && q % (EVERY ? EVERY : 1) == 0 && q / (EVERY ? EVERY : 1) < DA + DB) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        piece(q / (EVERY ? EVERY : 1));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[set][j], fa[set][i], acc[i][j], 0, 0, 0);
+            }
     };
 
     constexpr int FLY = (NBUF - 2) * (DA + DB);   // loads that may still be on their way when the next stage has to be there
 #pragma unroll
-    for (int s = 0; s < NBUF - 1; s++) fetch();
+    for (int s = 0; s < NBUF - 1; s++) {
+        fetch();
+        if (DMA && EVERY > 0) {
+#pragma unroll
+            for (int i = 0; i < DA + DB; i++) piece(i);
+        }
+    }
     commit();
     wait_dma_and_meet<FLY>();
     unsigned stage = 0;
@@ -200,7 +222,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
                 wait_dma_and_meet<FLY>();
                 read(0, next, 0);   // past the last whole stage: the tail's, or zeros
             }
-            multiply(kk & 1);
+            multiply(kk & 1, kk * FM * FN);
         }
         stage = next;
     }
@@ -217,7 +239,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
 #pragma unroll
                 for (int i = 0; i < FM; i++) fa[kk & 1][i][d] &= mask;
             }
-            multiply(kk & 1);
+            multiply(kk & 1, -1000);
         }
     }
     // The end of a tile.  w is the instruction's first operand, so a lane holds runs of four neighbouring n of one m: 32 rows of the

@@ -116,11 +116,11 @@ void launch_rowquant(const EngineView &v, const RowQuantArgs &a)
 }
 
 // Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.
-template <typename T, int BM, int BN, int BK, int NBUF, int WM, int WN, bool DMA = true>
+template <typename T, int BM, int BN, int NBUF, int WM, int WN, bool DMA, int EVERY>
 void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
 {
-    constexpr int bytes = (BM + BN) * BK * NBUF;
-    const auto kernel = linear_i8_tile_kernel<T, BM, BN, BK, NBUF, WM, WN, DMA>;
+    constexpr int bytes = (BM + BN) * 128 * NBUF;
+    const auto kernel = linear_i8_tile_kernel<T, BM, BN, 128, NBUF, WM, WN, DMA, EVERY>;
     static std::atomic<uint64_t> allowed{0};
     const uint64_t bit = 1ull << (v.device & 63);
     if (bytes > 65536 && !(allowed.load(std::memory_order_relaxed) & bit)) {
@@ -145,11 +145,11 @@ void launch_linear(const EngineView &v, const LinearI8Args &a)
         else if (a.m <= 16) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 1, false>), few_grid, dim3(512), 0, v.stream, a);
         else if (whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 2, true>), few_grid, dim3(512), 0, v.stream, a);
         else hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 2, false>), few_grid, dim3(512), 0, v.stream, a);
-    } else if (!whole) launch_linear_tiles<T, 128, 128, 128, 2, 2, 2, false>(v, a);
-    else if (variant == kLinear256) launch_linear_tiles<T, 256, 256, 128, 2, 2, 4>(v, a);
-    else if (variant == kLinear128) launch_linear_tiles<T, 128, 128, 128, 2, 2, 2>(v, a);
-    else if (variant == kLinear64Deep) launch_linear_tiles<T, 64, 64, 128, 4, 2, 2>(v, a);
-    else launch_linear_tiles<T, 64, 64, 128, 2, 2, 2>(v, a);
+    } else if (!whole) launch_linear_tiles<T, 128, 128, 2, 2, 2, false, 0>(v, a);
+    else if (variant == kLinear256) launch_linear_tiles<T, 256, 256, 2, 2, 4, true, 1>(v, a);
+    else if (variant == kLinear128) launch_linear_tiles<T, 128, 128, 2, 2, 2, true, 1>(v, a);
+    else if (variant == kLinear64Deep) launch_linear_tiles<T, 64, 64, 4, 2, 2, true, 0>(v, a);
+    else launch_linear_tiles<T, 64, 64, 2, 2, 2, true, 0>(v, a);
 }
 
 }  // namespace

@@ -1131,6 +1131,10 @@ static int engine_create(const void *model_bytes, size_t n, int device_id, int m
         e->err = "could not reserve LDS for conv12_fused_kernel";
         rc = APR_ERR_DEVICE;
     }
+    if (!rc && !operators_prepare()) {
+        e->err = "could not reserve LDS for linear_i8_tile_kernel";
+        rc = APR_ERR_DEVICE;
+    }
     {
         const char *genv = dev_getenv("APR_GRAPH");   // APR_GRAPH=0: small calls launch kernel by kernel too
         e->graph_on = !(genv && genv[0] == '0');

@@ -15,6 +15,8 @@ struct EngineView {
 bool engine_view(const apr_engine *e, EngineView &v) noexcept;
 // Keeps `text` as the engine's last error (this thread's, for a null handle) and returns `code`.
 int engine_fail(apr_engine *e, int code, const char *text) noexcept;
+// operators.hip, once for an engine, with its device current
+bool operators_prepare() noexcept;
 
 // Makes a device current for a scope and puts the caller's back: torch and other libraries in the process go by the current device.
 class DeviceScope {

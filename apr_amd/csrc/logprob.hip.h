@@ -104,6 +104,9 @@ struct ExpSum {
 // log of a sum of exponentials: 1 <= s, or 0, or NaN; the instruction's error is 2^-24 of log2 s or of 1
 __device__ __forceinline__ float log_of_sum(float s) { return __builtin_amdgcn_logf(s) * 0.69314718055994530942f; }
 
+// scale (x - m), also where x - m is beyond the largest float and the product is not (halves are exact, subnormals aside)
+__device__ __forceinline__ float scaled_distance(float x, float m, float scale) { return (0.5f * x - 0.5f * m) * (2.0f * scale); }
+
 // The outputs of a row from its sums and their logarithm; called by one lane.
 __device__ __forceinline__ void logprob_write(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, float x_target, bool has_target)
 {
@@ -113,13 +116,13 @@ __device__ __forceinline__ void logprob_write(const LogprobArgs &a, unsigned lon
         a.stat[2 * row + 1] = bad ? kNaN : log_s;
     }
     if (a.entropy) a.entropy[row] = bad ? kNaN : empty ? 0.0f : fmaxf(log_s - a.scale * (r.u * __builtin_amdgcn_rcpf(r.s)), 0.0f);
-    if (a.logprob) a.logprob[row] = !has_target ? 0.0f : bad ? kNaN : empty ? kNegInf : a.scale * (x_target - r.m) - log_s;
+    if (a.logprob) a.logprob[row] = !has_target ? 0.0f : bad ? kNaN : empty ? kNegInf : scaled_distance(x_target, r.m, a.scale) - log_s;
 }
 __device__ __forceinline__ void logprob_write_top(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, int place, unsigned long long key)
 {
     const bool bad = r.s != r.s, none = bad || !key;
     if (a.top_label) a.top_label[row * a.top + place] = none ? -1 : key_label(key);
-    if (a.top_logprob) a.top_logprob[row * a.top + place] = bad ? kNaN : none ? kNegInf : a.scale * (key_score(key) - r.m) - log_s;
+    if (a.top_logprob) a.top_logprob[row * a.top + place] = bad ? kNaN : none ? kNegInf : scaled_distance(key_score(key), r.m, a.scale) - log_s;
 }
 
 // ---- the best `top` of many keys, by one wave ----

@@ -5,7 +5,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <type_traits>
@@ -21,6 +20,7 @@ using namespace apr;
 namespace {
 
 constexpr size_t kMostRows = 0x7FFFFFFF, kMostStride = (size_t)1 << 40;
+constexpr double kLeastScale = 1e-30, kMostScale = 1e30;   // what is divided by it or multiplied with it stays in the range of a float
 constexpr unsigned kMostBlocks = 1u << 20;   // grids stride over their rows beyond that
 
 size_t element_size(int dtype) { return dtype == APR_F32 ? 4 : 2; }
@@ -115,20 +115,17 @@ void launch_rowquant(const EngineView &v, const RowQuantArgs &a)
     else launch(rowquant_kernel<T, 16, 8>, 1, 1024);
 }
 
-// Tiles of BM x BN outputs.  More than 64 KiB of LDS has to be allowed once on each device.
+// Tiles of BM x BN outputs
+template <typename T, int BM, int BN, int NBUF, int WM, int WN, bool DMA, int EVERY>
+constexpr auto linear_tiles() { return linear_i8_tile_kernel<T, BM, BN, 128, NBUF, WM, WN, DMA, EVERY>; }
+template <int BM, int BN, int NBUF>
+constexpr int kLinearLds = (BM + BN) * 128 * NBUF;
+
 template <typename T, int BM, int BN, int NBUF, int WM, int WN, bool DMA, int EVERY>
 void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
 {
-    constexpr int bytes = (BM + BN) * 128 * NBUF;
-    const auto kernel = linear_i8_tile_kernel<T, BM, BN, 128, NBUF, WM, WN, DMA, EVERY>;
-    static std::atomic<uint64_t> allowed{0};
-    const uint64_t bit = 1ull << (v.device & 63);
-    if (bytes > 65536 && !(allowed.load(std::memory_order_relaxed) & bit)) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return;
-        allowed.fetch_or(bit, std::memory_order_relaxed);
-    }
     const unsigned tiles_m = (a.m + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN;
-    hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n), dim3(WM * WN * 64), bytes, v.stream, a, tiles_m, tiles_n);
+    hipLaunchKernelGGL((linear_tiles<T, BM, BN, NBUF, WM, WN, DMA, EVERY>()), dim3(tiles_m * tiles_n), dim3(WM * WN * 64), (kLinearLds<BM, BN, NBUF>), v.stream, a, tiles_m, tiles_n);
 }
 
 template <typename T>
@@ -152,7 +149,22 @@ void launch_linear(const EngineView &v, const LinearI8Args &a)
     else launch_linear_tiles<T, 64, 64, 2, 2, 2, true, 0>(v, a);
 }
 
+template <typename T>
+bool allow_lds()
+{
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(linear_tiles<T, 256, 256, 2, 2, 4, true, 1>()), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               kLinearLds<256, 256, 2>) == hipSuccess;
+}
+
 }  // namespace
+
+namespace apr {
+
+// More than 64 KiB of LDS has to be allowed, once on each device; it loads this file's kernels there, too, so that the first call may
+// be one that is captured.
+bool operators_prepare() noexcept { return allow_lds<float>() && allow_lds<f16_t>() && allow_lds<bf16_t>(); }
+
+}  // namespace apr
 
 extern "C" {
 
@@ -170,7 +182,7 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
     if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
     if (n > kMostRows || n_labels < 1 || n_labels > kMostRows) return refuse(e, me, "1 <= n_labels < 2^31, n < 2^31");
     if (ld < n_labels || ld > kMostStride) return refuse(e, me, "ld is at least n_labels");
-    if (!(scale > 0.0) || !std::isfinite((float)scale) || (float)scale == 0.0f) return refuse(e, me, "scale is positive and finite");
+    if (!(scale >= kLeastScale && scale <= kMostScale)) return refuse(e, me, "1e-30 <= scale <= 1e30");
     if (top < 0 || top > APR_MAX_TOP) return refuse(e, me, "0 <= top <= APR_MAX_TOP");
     if (d_logprob && !d_target) return refuse(e, me, "d_logprob needs d_target");
     if (top == 0 && (d_top_label || d_top_logprob)) d_top_label = nullptr, d_top_logprob = nullptr;
@@ -203,7 +215,7 @@ int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_l
     if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
     if (n > kMostRows || n_labels < 1 || n_labels > kMostRows) return refuse(e, me, "1 <= n_labels < 2^31, n < 2^31");
     if (ld < n_labels || ld > kMostStride || ld_grad < n_labels || ld_grad > kMostStride) return refuse(e, me, "ld and ld_grad are at least n_labels");
-    if (!(scale > 0.0) || !std::isfinite((float)scale) || (float)scale == 0.0f) return refuse(e, me, "scale is positive and finite");
+    if (!(scale >= kLeastScale && scale <= kMostScale)) return refuse(e, me, "1e-30 <= scale <= 1e30");
     if (d_g_logprob && !d_target) return refuse(e, me, "d_g_logprob needs d_target");
     if (d_g_entropy && !d_entropy) return refuse(e, me, "d_g_entropy needs d_entropy");
     if (!n) return on_engine(e, me, [](const EngineView &) {});

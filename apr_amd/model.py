@@ -502,7 +502,9 @@ def windows_in(n_bytes: int, stride: int = BytesPerSecond) -> int:
 
 def _release(engine: Engine, addresses: List[int]) -> None:
     while addresses:
-        engine.device_free(addresses.pop())
+        p = addresses.pop()
+        if engine._fin.alive:   # a closed engine's handle is gone
+            engine.device_free(p)
 
 
 class LabelHead:

@@ -326,12 +326,14 @@ int apr_engine_num_features(const apr_engine *e);   /* 0 for a front-end-only en
  * Asynchronous on the engine's stream (inputs that another stream is still writing have to be waited for first:
  * apr_engine_stream); nothing is allocated and only kernels are launched, so a call may be captured into a graph.
  * The current device of the calling thread is left as it was.  Matrices are row-major with a row stride `ld` in elements;
- * what lies between the rows' ends is neither used nor written.  Zero rows are a no-op.
+ * what lies between the rows' ends is neither used nor written (rows are read in aligned units of 16 bytes, whose first and last may
+ * hold some of it).  Zero rows are a no-op.
  */
 
 /*
  * Log probabilities of given labels over rows of scores (APR_F32 / APR_F16 / APR_BF16), with entropy and best alternatives:
- * p = softmax(scale * logits) of each row, scale > 0 (1 / temperature); all sums in 32 bits, relative to the row's maximum.
+ * p = softmax(scale * logits) of each row, 1e-30 <= scale <= 1e30 (1 / temperature); all sums in 32 bits, relative to the row's
+ * maximum.
  *   d_target      [n]       label whose log probability is wanted; one outside [0, n_labels) names none: logprob 0
  *   d_logprob     [n]       log p[target]                              (needs d_target)
  *   d_entropy     [n]       -sum p log p, in nats

@@ -164,6 +164,19 @@ def test_logprobs_with_many_equal_scores(eng):
         assert got["top_label"][0].tolist() == list(range(32)) and got["top_label"][1].tolist() == (list(range(1, c, 2)) + list(range(0, c, 2)))[:32]
 
 
+@pytest.mark.parametrize("scale", [1e-30, 1e-10, 1e10, 1e30])
+@pytest.mark.parametrize("c", [60, 3000])
+def test_logprobs_at_the_ends_of_the_scale(eng, scale, c):
+    # scores of the size that the scale wants, one row with a label ruled out, one with the range's largest spread
+    g = torch.Generator(device=dev()).manual_seed(2)
+    x = torch.randn(4, c, generator=g, device=dev()) * 3.0 / scale
+    x[1, c // 2] = -INF
+    x[2, 0], x[2, 1:] = 3e38, -3e38
+    t = torch.randint(1, c, (4,), generator=g, device=dev(), dtype=torch.int32)
+    check(eng, x, t, top=3, scale=scale)
+    gradient_case(eng, x, t, scale, torch.full((4,), 1e-3, device=dev()), None)
+
+
 def test_logprobs_outputs_are_each_optional(eng):
     x, t = rows(5, 777, torch.float32, 3)
     want = run(eng, x, t, 4)
@@ -543,6 +556,7 @@ def test_label_head_on_the_engines_features(he_weights, clips):
     grad, gtol = oracle_l.gradient(z.float(), 1.0, torch.from_numpy(target).to(dev()), g)
     near(torch.from_numpy(r["d_logits"]).to(dev()), grad, gtol + 8 * slack[:, None] / n_used + 4 * o["tol_stat"][:, None] / n_used, "d_logits")
     assert np.array_equal(r["features"], f.cpu().numpy())
+    assert head.score(spec, top=0)["top_label"].shape == (10, 0) and head.score(spec[:0], target[:0])["entropy"].shape == (0,)
     again = head.score(spec, target, top=3)
     assert all(np.array_equal(again[k], got[k]) for k in got)
     assert np.array_equal(full.classify(spec)["logits"], cnn["logits"])     # the CNN's own head is as it was

@@ -36,12 +36,12 @@ def test_good_arguments_reach_the_engine(op):
     ("logprobs", dict(dtype=3)), ("logprobs", dict(dtype=-1)), ("logprobs", dict(c=0)), ("logprobs", dict(c=1 << 31, ld=1 << 31)),
     ("logprobs", dict(n=1 << 31)), ("logprobs", dict(ld=9)), ("logprobs", dict(ld=1 << 41)), ("logprobs", dict(scale=0.0)),
     ("logprobs", dict(scale=-1.0)), ("logprobs", dict(scale=float("nan"))), ("logprobs", dict(scale=float("inf"))),
-    ("logprobs", dict(scale=1e-60)), ("logprobs", dict(scale=1e39)), ("logprobs", dict(top=-1)), ("logprobs", dict(top=33)),
+    ("logprobs", dict(scale=1e-60)), ("logprobs", dict(scale=1e39)), ("logprobs", dict(scale=0.9e-30)), ("logprobs", dict(scale=1.1e30)), ("logprobs", dict(top=-1)), ("logprobs", dict(top=33)),
     ("logprobs", dict(target=None)), ("logprobs", dict(x=None)), ("logprobs", dict(x=P + 2)), ("logprobs", dict(dtype=1, x=P + 1)),
     ("logprobs", dict(target=P + 2)), ("logprobs", dict(lp=P + 1)), ("logprobs", dict(ent=P + 2)), ("logprobs", dict(stat=P + 2)),
     ("logprobs", dict(tl=P + 3)), ("logprobs", dict(tp=P + 2)),
     ("backward", dict(dtype=7)), ("backward", dict(c=0)), ("backward", dict(n=1 << 31)), ("backward", dict(ld=9)), ("backward", dict(ldg=9)),
-    ("backward", dict(scale=0.0)), ("backward", dict(scale=float("nan"))), ("backward", dict(target=None)), ("backward", dict(ent=None)),
+    ("backward", dict(scale=0.0)), ("backward", dict(scale=float("nan"))), ("backward", dict(scale=1e-31)), ("backward", dict(scale=1e31)), ("backward", dict(target=None)), ("backward", dict(ent=None)),
     ("backward", dict(x=None)), ("backward", dict(stat=None)), ("backward", dict(grad=None)), ("backward", dict(grad=P + 2)),
     ("backward", dict(grad=P, ldg=11)), ("backward", dict(g=P + 1)), ("backward", dict(h=P + 2)),
     ("quantize", dict(dtype=3)), ("quantize", dict(k=0)), ("quantize", dict(ld=9)), ("quantize", dict(ldq=9)), ("quantize", dict(x=None)),

@@ -64,8 +64,19 @@ __device__ __forceinline__ float wave_of_rows(float v, F f)
 template <typename F>
 __device__ __forceinline__ float wave_reduce(float v, F f) { return wave_of_rows(row_reduce(v, f), f); }
 
+// The sum of all lanes, wave-uniform: within the rows of 16, then a row's last lane to the next row, and lane 31 to the upper half
+__device__ __forceinline__ float wave_sum(float v)
+{
+    v = v + lane_move<0xB1>(v);
+    v = v + lane_move<0x4E>(v);
+    v = v + lane_move<0x141>(v);
+    v = v + lane_move<0x140>(v);
+    v = v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false));
+    v = v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 struct MaxOf { __device__ __forceinline__ float operator()(float p, float q) const { return fmaxf(p, q); } };
-struct SumOf { __device__ __forceinline__ float operator()(float p, float q) const { return p + q; } };
 
 constexpr float kLog2E = 1.44269504088896340736f;
 
@@ -143,15 +154,17 @@ __device__ __forceinline__ float reached_by(float v, int top)
     return key_score((unsigned long long)t << 32);
 }
 
-// Place of a lane's key among the first n lanes' keys, best first
-__device__ __forceinline__ int key_place(unsigned long long key, int n)
+// Place of a lane's key among the wave's first n, best first (n <= 64; the other lanes' keys are 0).  All lanes read them from LDS, two a time.
+__device__ __forceinline__ int key_place(unsigned long long key, int n, unsigned long long *list, int lane)
 {
+    list[lane] = key;
+    __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
     int place = 0;
-    const int lo = (int)(uint32_t)key, hi = (int)(uint32_t)(key >> 32);
-    for (int i = 0; i < n; i++) {
-        const unsigned long long other = ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, i);
-        place += other > key ? 1 : 0;
+    for (int i = 0; i < n; i += 4) {
+        const ulonglong2 p = *(const ulonglong2 *)(list + i), q = *(const ulonglong2 *)(list + i + 2);
+        place += (p.x > key ? 1 : 0) + (p.y > key ? 1 : 0) + (q.x > key ? 1 : 0) + (q.y > key ? 1 : 0);
     }
+    __builtin_amdgcn_wave_barrier();
     return place;
 }
 
@@ -198,9 +211,9 @@ __device__ __forceinline__ int keep_best(const unsigned long long (&k)[N], int t
 }
 
 // The alternatives of a row from at most 64 keys, one each of the first n lanes
-__device__ __forceinline__ void logprob_write_list(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, unsigned long long key, int n, int lane)
+__device__ __forceinline__ void logprob_write_list(const LogprobArgs &a, unsigned long long row, LogprobPart r, float log_s, unsigned long long key, int n, unsigned long long *list, int lane)
 {
-    const int place = key_place(key, n);
+    const int place = key_place(key, n, list, lane);
     if (lane < n && place < a.top) logprob_write_top(a, row, r, log_s, place, key);
     if (lane >= n && lane < a.top) logprob_write_top(a, row, r, log_s, lane, 0);
 }
@@ -267,6 +280,7 @@ struct Candidates {
             n += __builtin_popcountll(mask);
         }
     }
+    __device__ __forceinline__ unsigned long long *keys() const { return (unsigned long long *)list; }   // the list's place, when it is done with
     // at most 64 keys, one a lane (0: none)
     __device__ __forceinline__ unsigned long long finish(int top, int lane)
     {
@@ -284,7 +298,7 @@ struct Candidates {
 template <typename T, int E>
 __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
 {
-    __shared__ uint2 s_list[4][kList];
+    __shared__ __align__(16) uint2 s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (unsigned long long row = (unsigned long long)blockIdx.x * 4 + wave; row < a.n; row += (unsigned long long)gridDim.x * 4) {
         const T *x = (const T *)a.x + row * a.ld;
@@ -299,8 +313,8 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         ExpSum sum(r.m, a.scale);
 #pragma unroll
         for (int i = 0; i < E; i++) sum.add(v[i]);
-        r.s = wave_reduce(sum.s, SumOf());
-        r.u = wave_reduce(sum.u, SumOf());
+        r.s = wave_sum(sum.s);
+        r.u = wave_sum(sum.u);
         const float log_s = log_of_sum(r.s);
         const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
         float xt = 0.0f;
@@ -313,7 +327,7 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         c.least = reached_by(best, a.top);
         c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
         const unsigned long long key = c.finish(a.top, lane);
-        logprob_write_list(a, row, r, log_s, key, c.n, lane);
+        logprob_write_list(a, row, r, log_s, key, c.n, c.keys(), lane);
     }
 }
 
@@ -332,7 +346,7 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
 {
     constexpr int V = 16 / (int)sizeof(T), U = 16 / V;
     typedef T txv __attribute__((ext_vector_type(V)));
-    __shared__ uint2 s_list[4][kList];
+    __shared__ __align__(16) uint2 s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const unsigned long long works = a.n * a.pieces;
     const float c = a.scale * kLog2E, gap = kGap / a.scale, least_t = -200.0f / a.scale;
@@ -409,8 +423,8 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
         r.m = wave_reduce(m, MaxOf());
         // a reference of -inf: every score ruled out, or NaN in s
         const float d = ref == kNegInf ? 0.0f : ref - r.m, w = __builtin_amdgcn_exp2f(d * c);
-        s = wave_reduce(s, SumOf());
-        u = wave_reduce(u, SumOf());
+        s = wave_sum(s);
+        u = wave_sum(u);
         r.s = w * s;
         r.u = w * fmaf(fmaxf(d, least_t), s, u);
         const float log_s = log_of_sum(r.s);
@@ -425,9 +439,9 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
         if (!TOP) continue;
         const unsigned long long key = best.finish(a.top, lane);
         if (a.pieces == 1)
-            logprob_write_list(a, row, r, log_s, key, best.n, lane);
+            logprob_write_list(a, row, r, log_s, key, best.n, best.keys(), lane);
         else {
-            const int place = key_place(key, best.n);
+            const int place = key_place(key, best.n, best.keys(), lane);
             if (lane < best.n && place < a.top) a.part_top[work * a.top + place] = key;
             if (lane >= best.n && lane < a.top) a.part_top[work * a.top + lane] = 0;
         }
@@ -437,7 +451,7 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
 // ---- the pieces of a row joined, a wave per row ----
 __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int type)
 {
-    __shared__ unsigned long long s_list[64];
+    __shared__ __align__(16) unsigned long long s_list[64];
     const int lane = threadIdx.x;
     for (unsigned long long row = blockIdx.x; row < a.n; row += gridDim.x) {
         // the first 1024 keys of the pieces' lists: asked for before the sums are joined
@@ -471,8 +485,8 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
             s = fmaf(e, q.s, s);
             u = fmaf(e, fmaf(fmaxf(d, to.least), q.s, q.u), u);
         }
-        r.s = wave_reduce(s, SumOf());
-        r.u = wave_reduce(u, SumOf());
+        r.s = wave_sum(s);
+        r.u = wave_sum(u);
         const float log_s = log_of_sum(r.s);
         if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
@@ -510,7 +524,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
             n = keep_best(k, a.top, border, put);
         }
         __builtin_amdgcn_wave_barrier();
-        logprob_write_list(a, row, r, log_s, lane < n ? s_list[lane] : 0, n, lane);
+        logprob_write_list(a, row, r, log_s, lane < n ? s_list[lane] : 0, n, s_list, lane);
         __builtin_amdgcn_wave_barrier();
     }
 }

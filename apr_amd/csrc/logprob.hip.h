@@ -18,6 +18,7 @@
 namespace apr {
 
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kLowest = -3.402823466e+38f;   // of the finite ones
 constexpr float kNaN = __builtin_nanf("");
 
 // A score and its label as one whole number: larger is better, equal scores go to the lowest label, +0 and -0 are equal.
@@ -324,7 +325,8 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;
         Candidates c(s_list[wave]);
-        c.least = reached_by(best, a.top);
+        // the one best needs no search, and of a few labels all may be candidates
+        c.least = a.top == 1 ? fmaxf(r.m, kLowest) : a.n_labels <= 16 ? kLowest : reached_by(best, a.top);
         c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
         const unsigned long long key = c.finish(a.top, lane);
         logprob_write_list(a, row, r, log_s, key, c.n, c.keys(), lane);
@@ -539,16 +541,19 @@ struct LogprobPlan {
 // pieces, a round and a bit, 133).  A piece is a step at least, and the pieces' alternatives are as many as the join holds at once (one
 // row of 131071, 20 alternatives: 16 us in 33 pieces, 18 in 65, whose lists it takes in two goes, and 22 in 17).
 constexpr size_t kWavesWanted = 3200, kStep = 1024, kJoined = 1024;
+// Up to here a row is not cut: 2000 scores take 5.6 us as one and 8.7 as two pieces and their join, 4000 8.3 and 8.7, 6000 9.9 and 9.0.
+constexpr size_t kWhole = 4096;
 inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
 {
     LogprobPlan p = {0, 1, (unsigned)c, 0};
-    if (c <= 1024) {
+    if (c <= kStep) {
         p.each = (int)((c + 63) / 64);
         return p;
     }
     // pieces while the rows alone are too few waves
     size_t pieces = std::min((kWavesWanted + n - 1) / std::max<size_t>(n, 1), (c + kStep - 1) / kStep);
     if (top > 0) pieces = std::min(pieces, kJoined / (size_t)top);
+    if (c <= kWhole) pieces = 1;
     p.piece_len = (unsigned)(((c + pieces - 1) / pieces + 7) / 8 * 8);
     p.pieces = (unsigned)((c + p.piece_len - 1) / p.piece_len);
     if (p.pieces > 1) p.work = n * p.pieces * (size_t)top * 8 + (n * p.pieces * sizeof(LogprobPart) + 15) / 16 * 16;

@@ -155,6 +155,8 @@ __device__ __forceinline__ float reached_by(float v, int top)
     return key_score((unsigned long long)t << 32);
 }
 
+typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+
 // Place of a lane's key among the wave's first n, best first (n <= 64; the other lanes' keys are 0).  All lanes read them from LDS, two a time.
 __device__ __forceinline__ int key_place(unsigned long long key, int n, unsigned long long *list, int lane)
 {
@@ -162,7 +164,7 @@ __device__ __forceinline__ int key_place(unsigned long long key, int n, unsigned
     __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
     int place = 0;
     for (int i = 0; i < n; i += 4) {
-        const ulonglong2 p = *(const ulonglong2 *)(list + i), q = *(const ulonglong2 *)(list + i + 2);
+        const u64x2 p = *(const u64x2 *)(list + i), q = *(const u64x2 *)(list + i + 2);
         place += (p.x > key ? 1 : 0) + (p.y > key ? 1 : 0) + (q.x > key ? 1 : 0) + (q.y > key ? 1 : 0);
     }
     __builtin_amdgcn_wave_barrier();
@@ -221,20 +223,20 @@ __device__ __forceinline__ void logprob_write_list(const LogprobArgs &a, unsigne
 
 // A wave's candidates for the alternatives, collected in LDS as its scores come by.  Taken are scores of at least `least`; when the list
 // is full, the best are kept and `least` rises.  If equal scores still are too many, they are taken one by one, and only those whose key
-// passes `border`.  An entry is the score's bits and the label; keys are made of them when the list is looked at, which is much rarer.
+// passes `border`.  An entry is the score's bits above the label; keys are made of them when the list is looked at, which is much rarer.
 constexpr int kList = 128;
 struct Candidates {
-    uint2 *list;
+    unsigned long long *list;
     unsigned long long border = 0;
     int n = 0;
     float least = __builtin_inff();
-    __device__ __forceinline__ explicit Candidates(uint2 *l) : list(l) {}
+    __device__ __forceinline__ explicit Candidates(unsigned long long *l) : list(l) {}
     __device__ __forceinline__ unsigned long long key_at(int i) const
     {
         if (i >= n) return 0;
-        const uint2 v = list[i];
-        return score_key(__builtin_bit_cast(float, v.x), v.y);
+        return score_key(__builtin_bit_cast(float, (uint32_t)(list[i] >> 32)), (unsigned)list[i]);
     }
+    static __device__ __forceinline__ unsigned long long entry(float v, unsigned label) { return (unsigned long long)__builtin_bit_cast(uint32_t, v) << 32 | label; }
     __device__ __forceinline__ void shrink(int top, int lane)
     {
         __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
@@ -242,7 +244,7 @@ struct Candidates {
 #pragma unroll
         for (int i = 0; i < kList / 64; i++) k[i] = key_at(64 * i + lane);
         __builtin_amdgcn_wave_barrier();
-        n = keep_best(k, top, border, [&](int at, unsigned long long key) { list[at] = make_uint2(__builtin_bit_cast(uint32_t, key_score(key)), (unsigned)key_label(key)); });
+        n = keep_best(k, top, border, [&](int at, unsigned long long key) { list[at] = entry(key_score(key), (unsigned)key_label(key)); });
         least = fmaxf(least, key_score(border));
         __builtin_amdgcn_wave_barrier();
     }
@@ -260,7 +262,7 @@ struct Candidates {
                     for (int i = 0; i < N; i++) {
                         const unsigned long long mask = __ballot(v[i] >= least);
                         if (!mask) continue;
-                        if (mask >> lane & 1) list[n + below(mask)] = make_uint2(__builtin_bit_cast(uint32_t, v[i]), label(i));
+                        if (mask >> lane & 1) list[n + below(mask)] = entry(v[i], label(i));
                         n += __builtin_popcountll(mask);
                     }
                 }
@@ -277,11 +279,10 @@ struct Candidates {
                 shrink(top, lane);
                 mask = __ballot(y >= least && score_key(y, label(i)) >= border);
             }
-            if (mask >> lane & 1) list[n + below(mask)] = make_uint2(__builtin_bit_cast(uint32_t, y), label(i));
+            if (mask >> lane & 1) list[n + below(mask)] = entry(y, label(i));
             n += __builtin_popcountll(mask);
         }
     }
-    __device__ __forceinline__ unsigned long long *keys() const { return (unsigned long long *)list; }   // the list's place, when it is done with
     // at most 64 keys, one a lane (0: none)
     __device__ __forceinline__ unsigned long long finish(int top, int lane)
     {
@@ -296,10 +297,11 @@ struct Candidates {
 // ---- short rows: a wave per row, E scores a lane ----
 //
 // Candidates for the alternatives are the scores that at least `top` lanes' best scores reach: about as many as are wanted.
+// Bound by instruction issue: 35999 x 527 bf16 takes 15.6 us without alternatives and 23.3 with five (38 MB: 8.4 us at the rate of a copy).
 template <typename T, int E>
 __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
 {
-    __shared__ __align__(16) uint2 s_list[4][kList];
+    __shared__ __align__(16) unsigned long long s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (unsigned long long row = (unsigned long long)blockIdx.x * 4 + wave; row < a.n; row += (unsigned long long)gridDim.x * 4) {
         const T *x = (const T *)a.x + row * a.ld;
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
         c.least = a.top == 1 ? fmaxf(r.m, kLowest) : a.n_labels <= 16 ? kLowest : reached_by(best, a.top);
         c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
         const unsigned long long key = c.finish(a.top, lane);
-        logprob_write_list(a, row, r, log_s, key, c.n, c.keys(), lane);
+        logprob_write_list(a, row, r, log_s, key, c.n, c.list, lane);
     }
 }
 
@@ -340,15 +342,17 @@ __global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
 // maximum itself would be new in some lane at nearly every step.  A step's 16 terms of a lane are summed before they are added.
 // 16-byte loads begin at the 16-byte unit that the piece begins in (which is inside the allocation, as the piece's first element is);
 // what does not belong to the piece counts as ruled out.
+// HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us, 5.4 TB/s (141 with 20 alternatives); a workgroup per row, whose waves meet
+// three times a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 13.7 us in 50 pieces a row.
 constexpr float kGap = 8.0f;
 
-// TOP: with alternatives, whose code takes registers (98 of them: five waves a SIMD instead of eight).
+// TOP: with alternatives, whose code takes registers (85 to 93: five waves a SIMD instead of eight).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(LogprobArgs a)
 {
     constexpr int V = 16 / (int)sizeof(T), U = 16 / V;
     typedef T txv __attribute__((ext_vector_type(V)));
-    __shared__ __align__(16) uint2 s_list[4][kList];
+    __shared__ __align__(16) unsigned long long s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const unsigned long long works = a.n * a.pieces;
     const float c = a.scale * kLog2E, gap = kGap / a.scale, least_t = -200.0f / a.scale;
@@ -441,23 +445,24 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
         if (!TOP) continue;
         const unsigned long long key = best.finish(a.top, lane);
         if (a.pieces == 1)
-            logprob_write_list(a, row, r, log_s, key, best.n, best.keys(), lane);
+            logprob_write_list(a, row, r, log_s, key, best.n, best.list, lane);
         else {
-            const int place = key_place(key, best.n, best.keys(), lane);
+            const int place = key_place(key, best.n, best.list, lane);
             if (lane < best.n && place < a.top) a.part_top[work * a.top + place] = key;
             if (lane >= best.n && lane < a.top) a.part_top[work * a.top + lane] = 0;
         }
     }
 }
 
-// ---- the pieces of a row joined, a wave per row ----
+// ---- the pieces of a row joined, a wave per row: 4.9 us for one row, 5.4 for 64, most of it the launch and two loads in a row ----
 __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int type)
 {
     __shared__ __align__(16) unsigned long long s_list[64];
     const int lane = threadIdx.x;
     for (unsigned long long row = blockIdx.x; row < a.n; row += gridDim.x) {
-        // the first 1024 keys of the pieces' lists: asked for before the sums are joined
-        const unsigned long long *keys = a.part_top + row * a.pieces * a.top, all = (unsigned long long)a.pieces * a.top;
+        // the pieces' lists, at most 1024 keys (logprob_plan): asked for before the sums are joined
+        const unsigned long long *keys = a.part_top + row * a.pieces * a.top;
+        const unsigned all = a.pieces * a.top;
         unsigned long long k[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) k[i] = 64u * i + lane < all ? keys[64 * i + lane] : 0;
@@ -514,17 +519,6 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
             }
         } else
             n = keep_best(k, a.top, border, put);
-        for (unsigned long long k0 = 1024; k0 < all; k0 += 960) {   // more pieces: with the best so far in the first place
-            __builtin_amdgcn_wave_barrier();
-            k[0] = lane < n ? s_list[lane] : 0;
-#pragma unroll
-            for (int i = 1; i < 16; i++) {
-                const unsigned long long at = k0 + 64 * (i - 1) + lane;
-                k[i] = at < all ? keys[at] : 0;
-            }
-            __builtin_amdgcn_wave_barrier();
-            n = keep_best(k, a.top, border, put);
-        }
         __builtin_amdgcn_wave_barrier();
         logprob_write_list(a, row, r, log_s, lane < n ? s_list[lane] : 0, n, s_list, lane);
         __builtin_amdgcn_wave_barrier();
@@ -540,7 +534,7 @@ struct LogprobPlan {
 // Waves that fill the chip in one round (the form with alternatives has places for 5120: 2000 rows in two pieces take 116 us, in three
 // pieces, a round and a bit, 133).  A piece is a step at least, and the pieces' alternatives are as many as the join holds at once (one
 // row of 131071, 20 alternatives: 16 us in 33 pieces, 18 in 65, whose lists it takes in two goes, and 22 in 17).
-constexpr size_t kWavesWanted = 3200, kStep = 1024, kJoined = 1024;
+constexpr size_t kWavesWanted = 3200, kStep = 1024, kJoined = 16 * 64;   // kJoined: k of logprob_join_kernel
 // Up to here a row is not cut: 2000 scores take 5.6 us as one and 8.7 as two pieces and their join, 4000 8.3 and 8.7, 6000 9.9 and 9.0.
 constexpr size_t kWhole = 4096;
 inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
@@ -575,6 +569,7 @@ struct LogprobGradArgs {
 // lane, so grad may be x.  Stores are whole 16-byte units of grad, wherever its rows begin (what a row has before its first
 // and behind its last whole unit goes element by element); the loads follow them at whatever alignment x has then, which the hardware takes.
 // p = exp2(scale log2 e (x - m) - log2 e log s): x - m is exact for the scores that matter, the rest rounds once.
+// HBM-bound: 8192 x 32000 bf16 takes 234 us, 4.5 TB/s (a large copy: 4.7), 509 x 50257 f32 53 us, 3.8 TB/s.
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(256) void logprob_grad_kernel(LogprobGradArgs a)
 {

@@ -31,7 +31,8 @@ struct RowQuantArgs {
     unsigned k;
 };
 
-// G waves per row, U units of 16 bytes a lane in registers, read once (a row that is longer than that is read twice).  HBM-bound.  16-byte loads
+// G waves per row, U units of 16 bytes a lane in registers, read once (a row that is longer than that is read twice).
+// HBM-bound: 35999 x 1024 f32 takes 42 us, 4.4 TB/s (a large copy: 4.7), 4096 x 8191 bf16 27 us, 3.8 TB/s.  16-byte loads
 // begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is); what does not belong
 // to the row counts as 0 and is not written.  A lane writes the 4 or 8 values of its unit together, at whatever alignment they have.
 template <typename T, int G, int U>

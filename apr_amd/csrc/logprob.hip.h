@@ -13,6 +13,7 @@
 
 #include <algorithm>
 
+#include "../../include/apr.h"
 #include "element.hip.h"
 
 namespace apr {
@@ -65,17 +66,44 @@ __device__ __forceinline__ float wave_of_rows(float v, F f)
 template <typename F>
 __device__ __forceinline__ float wave_reduce(float v, F f) { return wave_of_rows(row_reduce(v, f), f); }
 
-// The sum of all lanes, wave-uniform: within the rows of 16, then a row's last lane to the next row, and lane 31 to the upper half
-__device__ __forceinline__ float wave_sum(float v)
+// The sums of two values over all lanes, wave-uniform.  The first step leaves p's in the lower and q's in the upper half of one register.
+__device__ __forceinline__ void wave_sums(float &p, float &q)
 {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    const auto both = [](u32x2 v) {
+        const unsigned lower = v.x, upper = v.y;   // by value: a bit cast of an element itself takes the first one
+        return __builtin_bit_cast(float, lower) + __builtin_bit_cast(float, upper);
+    };
+    float v = both(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, p), __builtin_bit_cast(unsigned, q), false, false));
     v = v + lane_move<0xB1>(v);
     v = v + lane_move<0x4E>(v);
     v = v + lane_move<0x141>(v);
     v = v + lane_move<0x140>(v);
-    v = v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false));
-    v = v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false));
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+    const unsigned b = __builtin_bit_cast(unsigned, v);
+    const int w = __builtin_bit_cast(int, both(__builtin_amdgcn_permlane16_swap(b, b, false, false)));
+    p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(w, 0));
+    q = __builtin_bit_cast(float, __builtin_amdgcn_readlane(w, 32));
 }
+
+// The largest of all lanes, wave-uniform, as whole numbers, whose maximum folds with the move (a float's is made quiet first)
+__device__ __forceinline__ int wave_max(int v)
+{
+    const int none = (int)0x80000000;
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));   // a row's last lane to the next row
+    v = max(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));   // lane 31 to the upper half
+    return __builtin_amdgcn_readlane(v, 63);
+}
+// A float as a whole number of the same order, and back
+__device__ __forceinline__ int ordered(float v)
+{
+    const int b = __builtin_bit_cast(int, v);
+    return b ^ (b >> 31 & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float of_ordered(int b) { return __builtin_bit_cast(float, b ^ (b >> 31 & 0x7FFFFFFF)); }
 
 struct MaxOf { __device__ __forceinline__ float operator()(float p, float q) const { return fmaxf(p, q); } };
 
@@ -95,6 +123,8 @@ struct LogprobArgs {
     struct LogprobPart *part;
     unsigned long long *part_top;   // [row][piece][top], best first, 0 = none
     unsigned pieces, piece_len;
+    // short rows: a wave's, at most kRows, and 65536 / top rounded up
+    unsigned rows, per_top;
 };
 
 // Sums of a piece of a row relative to its own maximum m (as a score): s = sum exp(scale (x - m)), u = sum exp(..) (x - m).
@@ -142,9 +172,8 @@ __device__ __forceinline__ void logprob_write_top(const LogprobArgs &a, unsigned
 // A score that at least `top` of the wave's 64 values reach: the binary search over the ordered bits counts lanes with a ballot.  The
 // highest 16 bits are enough, a score that is a little lower lets a few more candidates through.  Never below the lowest finite
 // score: what is ruled out is no candidate.
-__device__ __forceinline__ float reached_by(float v, int top)
+__device__ __forceinline__ float reached_by(uint32_t k, int top)
 {
-    const uint32_t k = (uint32_t)(score_key(v, 0) >> 32);
     uint32_t t = 0;
 #pragma unroll
     for (int b = 31; b >= 16; b--) {
@@ -154,6 +183,7 @@ __device__ __forceinline__ float reached_by(float v, int top)
     t = t < 0x00800000u ? 0x00800000u : t;
     return key_score((unsigned long long)t << 32);
 }
+__device__ __forceinline__ float reached_by(float v, int top) { return reached_by((uint32_t)(score_key(v, 0) >> 32), top); }
 
 typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
 
@@ -294,44 +324,77 @@ struct Candidates {
     }
 };
 
-// ---- short rows: a wave per row, E scores a lane ----
+// ---- short rows: a wave holds a row, E scores a lane, one row after the other ----
 //
 // Candidates for the alternatives are the scores that at least `top` lanes' best scores reach: about as many as are wanted.
-// Bound by instruction issue: 35999 x 527 bf16 takes 15.6 us without alternatives and 23.3 with five (38 MB: 8.4 us at the rate of a copy).
+// Bound by instruction issue, so what belongs to a row and not to its scores is done by a lane for each of the wave's rows, at the end.
+// 35999 x 527 bf16 takes 12.8 us without alternatives and 22.1 with five (38 MB: 8.4 us at the rate of a copy); a row at a time 15.3 and
+// 24.4, and 100000 x 64 f32 with five 31 against 37.  Eight rows a wave are no faster, and while they leave waves unused much slower.
+constexpr unsigned kRows = 4;
 template <typename T, int E>
-__global__ __launch_bounds__(256, 8) void logprob_wave_kernel(LogprobArgs a)
+__global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(LogprobArgs a)
 {
-    __shared__ __align__(16) unsigned long long s_list[4][kList];
+    __shared__ __align__(16) unsigned long long s_list[4][kList], s_top[4][kRows * APR_MAX_TOP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (unsigned long long row = (unsigned long long)blockIdx.x * 4 + wave; row < a.n; row += (unsigned long long)gridDim.x * 4) {
-        const T *x = (const T *)a.x + row * a.ld;
-        float v[E], best = kNegInf;
+    for (unsigned long long row0 = ((unsigned long long)blockIdx.x * 4 + wave) * a.rows; row0 < a.n; row0 += (unsigned long long)gridDim.x * 4 * a.rows) {
+        const unsigned rows = (unsigned)min((unsigned long long)a.rows, a.n - row0);
+        const int targets = a.target && (unsigned)lane < rows ? a.target[row0 + lane] : -1;
+        LogprobPart mine = {0.0f, 0.0f, 0.0f};   // lane i: row i's
+        T mine_t = (T)0.0f;
+        const bool has_t = (unsigned)targets < a.n_labels;
+        for (unsigned i_row = 0; i_row < rows; i_row++) {
+            const T *x = (const T *)a.x + (row0 + i_row) * a.ld;
+            float v[E], best = kNegInf;
 #pragma unroll
-        for (int i = 0; i < E; i++) v[i] = i < E - 1 || 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf;
-        const int t = a.target ? __builtin_amdgcn_readfirstlane(a.target[row]) : -1;
+            for (int i = 0; i < E; i++) v[i] = i < E - 1 || 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf;
+            if (i_row == 0 && has_t) mine_t = x[lane * a.ld + (unsigned)targets];   // behind the first row's loads, not before them
 #pragma unroll
-        for (int i = 0; i < E; i++) best = fmaxf(best, v[i]);
-        LogprobPart r;
-        r.m = wave_reduce(best, MaxOf());
-        ExpSum sum(r.m, a.scale);
+            for (int i = 0; i < E; i++) best = fmaxf(best, v[i]);
+            const int key_best = ordered(best);
+            LogprobPart r;
+            r.m = of_ordered(wave_max(key_best));
+            ExpSum sum(r.m, a.scale);
 #pragma unroll
-        for (int i = 0; i < E; i++) sum.add(v[i]);
-        r.s = wave_sum(sum.s);
-        r.u = wave_sum(sum.u);
-        const float log_s = log_of_sum(r.s);
-        const bool has_t = t >= 0 && (unsigned)t < a.n_labels;
-        float xt = 0.0f;
+            for (int i = 0; i < E; i++) sum.add(v[i]);
+            wave_sums(sum.s, sum.u);
+            const bool me = (unsigned)lane == i_row;
+            mine.m = me ? r.m : mine.m;
+            mine.s = me ? sum.s : mine.s;
+            mine.u = me ? sum.u : mine.u;
+            if (!a.top) continue;
+            if (a.top == 1) {   // the lowest label that has the row's maximum
+                unsigned label = 0;
 #pragma unroll
-        for (int i = 0; i < E; i++)
-            if (has_t && t >> 6 == i) xt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[i]), t & 63));
-        if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
+                for (int i = E - 1; i >= 0; i--) {
+                    const unsigned long long mask = __ballot(v[i] == r.m);
+                    if (mask) label = 64 * i + __builtin_ctzll(mask);
+                }
+                if (lane == 0) s_top[wave][i_row] = r.m == kNegInf ? 0 : score_key(r.m, label);
+                continue;
+            }
+            Candidates c(s_list[wave]);
+            // of a few labels all may be candidates
+            c.least = a.n_labels <= 16 ? kLowest : reached_by((uint32_t)key_best ^ 0x80000000u, a.top);
+            c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
+            const unsigned long long key = c.finish(a.top, lane);
+            const int place = key_place(key, c.n, c.list, lane);
+            unsigned long long *to = s_top[wave] + i_row * a.top;
+            if (lane < c.n && place < a.top) to[place] = key;
+            if (lane >= c.n && lane < a.top) to[lane] = 0;
+        }
+        const float log_s = log_of_sum(mine.s);
+        if ((unsigned)lane < rows) logprob_write(a, row0 + lane, mine, log_s, to_f32(mine_t), has_t);
         if (!a.top) continue;
-        Candidates c(s_list[wave]);
-        // the one best needs no search, and of a few labels all may be candidates
-        c.least = a.top == 1 ? fmaxf(r.m, kLowest) : a.n_labels <= 16 ? kLowest : reached_by(best, a.top);
-        c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
-        const unsigned long long key = c.finish(a.top, lane);
-        logprob_write_list(a, row, r, log_s, key, c.n, c.list, lane);
+        __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
+        for (unsigned i = lane; i < (rows * a.top + 63u & ~63u); i += 64) {   // every lane, as they read each other's rows
+            const unsigned i_row = min(i * a.per_top >> 16, rows - 1);
+            LogprobPart r;
+            r.m = __shfl(mine.m, i_row);
+            r.s = __shfl(mine.s, i_row);
+            const float l = __shfl(log_s, i_row);
+            if (i < rows * a.top) logprob_write_top(a, row0, r, l, i, s_top[wave][i]);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -429,8 +492,7 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
         r.m = wave_reduce(m, MaxOf());
         // a reference of -inf: every score ruled out, or NaN in s
         const float d = ref == kNegInf ? 0.0f : ref - r.m, w = __builtin_amdgcn_exp2f(d * c);
-        s = wave_sum(s);
-        u = wave_sum(u);
+        wave_sums(s, u);
         r.s = w * s;
         r.u = w * fmaf(fmaxf(d, least_t), s, u);
         const float log_s = log_of_sum(r.s);
@@ -492,8 +554,9 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
             s = fmaf(e, q.s, s);
             u = fmaf(e, fmaf(fmaxf(d, to.least), q.s, q.u), u);
         }
-        r.s = wave_sum(s);
-        r.u = wave_sum(u);
+        wave_sums(s, u);
+        r.s = s;
+        r.u = u;
         const float log_s = log_of_sum(r.s);
         if (lane == 0) logprob_write(a, row, r, log_s, xt, has_t);
         if (!a.top) continue;

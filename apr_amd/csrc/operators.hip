@@ -67,7 +67,8 @@ template <typename T>
 void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPlan &p)
 {
     if (p.each) {
-        const dim3 grid((unsigned)std::min<unsigned long long>((a.n + 3) / 4, kMostBlocks)), block(256);
+        const unsigned rows = 4 * a.rows;
+        const dim3 grid((unsigned)std::min<unsigned long long>((a.n + rows - 1) / rows, kMostBlocks)), block(256);
         const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, v.stream, a); };
         switch (p.each) {   // scores a lane: what a row has beyond them is computed for nothing
         case 1: return launch(logprob_wave_kernel<T, 1>);
@@ -201,7 +202,10 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
     a.pieces = plan.pieces; a.piece_len = plan.piece_len;
     a.part_top = (unsigned long long *)d_work;
     a.part = (LogprobPart *)((char *)d_work + (plan.pieces > 1 ? n * plan.pieces * (size_t)top * 8 : 0));
+    a.per_top = top ? (65536u + top - 1) / top : 0;
     return on_engine(e, me, [&](const EngineView &v) {
+        // 32 waves fit a CU: a wave takes a row until the chip is full
+        a.rows = (unsigned)std::max<size_t>(1, std::min<size_t>(kRows, n / (32 * (size_t)v.n_cus)));
         with_type(dtype, [&](auto *p) { launch_logprobs<APR_TYPE_OF(p)>(v, a, plan); });
         if (plan.pieces > 1) hipLaunchKernelGGL(logprob_join_kernel, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(64), 0, v.stream, a, dtype);
     });

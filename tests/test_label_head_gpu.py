@@ -115,6 +115,19 @@ def test_logprobs_over_row_counts(eng, n, c, dtype):
     check(eng, x, t, top=3)
 
 
+@pytest.mark.parametrize("n,c,top", [(16385, 700, 5), (20001, 64, 32), (24577, 527, 0), (35999, 100, 1), (36003, 17, 3), (140002, 3, 2), (140003, 40, 31)])
+def test_logprobs_of_many_rows(eng, n, c, top):
+    # several rows to a wave, the last wave's rows cut short; some without labels, some of NaN, between the others
+    for dtype in (torch.float32, torch.bfloat16):
+        x, t = rows(n, c, dtype, n, masked=0.05, ld=c + 5)
+        x[5::37] = -INF
+        x[n - 1] = -INF
+        x[7::41, c // 2] = float("nan")
+        x[9::43] = 0.5
+        t[::11], t[3::13] = -1, c
+        check(eng, x, t, top=top)
+
+
 @pytest.mark.parametrize("top", [0, 1, 2, 3, 7, 8, 16, 31, 32])
 @pytest.mark.parametrize("c", [5, 64, 700, 9000, 100000])
 def test_logprobs_top_counts(eng, top, c):

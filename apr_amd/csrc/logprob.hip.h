@@ -403,13 +403,13 @@ __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(Logpr
 // No lane waits for another wave.  The sums are relative to a reference that the wave shares: the best score so far, renewed only
 // when a score passes it by more than kGap (then exp <= e^kGap, and nothing is lost: the sums are floating point), because the running
 // maximum itself would be new in some lane at nearly every step.  A step's 16 terms of a lane are summed before they are added.
-// 16-byte loads begin at the 16-byte unit that the piece begins in (which is inside the allocation, as the piece's first element is);
-// what does not belong to the piece counts as ruled out.
+// 16-byte loads begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is);
+// what does not belong to the row counts as ruled out.
 // HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us, 5.4 TB/s (141 with 20 alternatives); a workgroup per row, whose waves meet
-// three times a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 13.7 us in 50 pieces a row.
+// three times a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 11.9 us in 64 pieces a row.
 constexpr float kGap = 8.0f;
 
-// TOP: with alternatives, whose code takes registers (85 to 93: five waves a SIMD instead of eight).
+// TOP: with alternatives, whose code takes registers (95: five waves a SIMD instead of eight).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(LogprobArgs a)
 {
@@ -421,9 +421,11 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
     const float c = a.scale * kLog2E, gap = kGap / a.scale, least_t = -200.0f / a.scale;
     for (unsigned long long work = (unsigned long long)blockIdx.x * waves + wave; work < works; work += (unsigned long long)gridDim.x * waves) {
         const unsigned long long row = a.pieces == 1 ? work : work / a.pieces;
-        const unsigned piece = (unsigned)(work - row * a.pieces), j0 = piece * a.piece_len, j1 = min(j0 + a.piece_len, a.n_labels);
+        const unsigned piece = (unsigned)(work - row * a.pieces);
         const T *x = (const T *)a.x + row * a.ld;
-        const unsigned off = (unsigned)(((unsigned long long)(x + j0) & 15) / sizeof(T));
+        // all pieces but the first begin with a 16-byte unit, so that none but the last takes a step for what a unit holds of its neighbour
+        const unsigned out = (unsigned)(((unsigned long long)x & 15) / sizeof(T)), off = piece ? 0 : out;
+        const unsigned j0 = piece ? piece * a.piece_len - out : 0, j1 = piece + 1 < a.pieces ? (piece + 1) * a.piece_len - out : a.n_labels;
         const txv *units = (const txv *)(x + j0 - off);
         const unsigned len = j1 - j0 + off, n_units = (len + V - 1) / V, steps = (n_units + 64 * U - 1) / (64 * U);
         const unsigned keep = len - (n_units - 1) * V;   // elements of the last unit
@@ -516,18 +518,30 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
     }
 }
 
-// ---- the pieces of a row joined, a wave per row: 4.9 us for one row, 5.4 for 64, most of it the launch and two loads in a row ----
+constexpr unsigned kJoined = 1024, kHeads = 8;
+static_assert(2 * kHeads == kJoined / 64, "one set of registers for both");
+
+// ---- the pieces of a row joined, a wave per row: 5.3 us for one row, 5.5 for 64, most of it the launch and two loads in a row ----
 __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int type)
 {
     __shared__ __align__(16) unsigned long long s_list[64];
     const int lane = threadIdx.x;
     for (unsigned long long row = blockIdx.x; row < a.n; row += gridDim.x) {
-        // the pieces' lists, at most 1024 keys (logprob_plan): asked for before the sums are joined
+        // The pieces' lists, asked for before the sums are joined: all their keys where those are 1024 at most, otherwise the best kHeads of
+        // each of at most 128 pieces (logprob_plan), lane i's and i + 64's.
         const unsigned long long *keys = a.part_top + row * a.pieces * a.top;
         const unsigned all = a.pieces * a.top;
-        unsigned long long k[16];
+        unsigned long long k[kJoined / 64];
+        if (all <= kJoined) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) k[i] = 64u * i + lane < all ? keys[64 * i + lane] : 0;
+            for (unsigned i = 0; i < kJoined / 64; i++) k[i] = 64u * i + lane < all ? keys[64 * i + lane] : 0;
+        } else {
+#pragma unroll
+            for (unsigned i = 0; i < 2 * kHeads; i++) {
+                const unsigned p = lane + i / kHeads * 64;
+                k[i] = p < a.pieces ? keys[p * a.top + i % kHeads] : 0;
+            }
+        }
         unsigned long long sample = 0;
         if (a.top && a.pieces < 64) {
             const unsigned each = 64 / a.pieces, p = lane / each, j = lane - p * each;
@@ -566,16 +580,26 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int typ
         const auto put = [&](int at, unsigned long long key) { s_list[at] = key; };
         const float least = reached_by(sample ? key_score(sample) : kNegInf, a.top);
         const unsigned long long reach = score_key(least, 0) >> 32 << 32;
+        const bool behind = all > kJoined && (k[kHeads - 1] >= reach || k[2 * kHeads - 1] >= reach);   // the heads' last ones count, so what is behind them may
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (unsigned i = 0; i < kJoined / 64; i++) {
             if (k[i] < reach) k[i] = 0;
             n += __builtin_popcountll(__ballot(k[i] != 0));
         }
-        if (n <= 64) {
+        if (__ballot(behind)) {
+            // some piece holds many of the best: all keys, 64 at a time, to what is kept of those before
+            n = 0;
+            for (unsigned i = 0; i < all; i += 64) {
+                const unsigned long long two[2] = {lane < n ? s_list[lane] : 0, i + lane < all ? keys[i + lane] : 0};
+                __builtin_amdgcn_wave_barrier();
+                n = keep_best(two, a.top, border, put);
+                __builtin_amdgcn_wave_barrier();
+            }
+        } else if (n <= 64) {
             n = 0;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
+            for (unsigned i = 0; i < kJoined / 64; i++) {
                 const unsigned long long mask = __ballot(k[i] != 0);
                 if (k[i]) put(n + below(mask), k[i]);
                 n += __builtin_popcountll(mask);
@@ -594,10 +618,11 @@ struct LogprobPlan {
     unsigned pieces, piece_len;
     size_t work;   // bytes
 };
-// Waves that fill the chip in one round (the form with alternatives has places for 5120: 2000 rows in two pieces take 116 us, in three
-// pieces, a round and a bit, 133).  A piece is a step at least, and the pieces' alternatives are as many as the join holds at once (one
-// row of 131071, 20 alternatives: 16 us in 33 pieces, 18 in 65, whose lists it takes in two goes, and 22 in 17).
-constexpr size_t kWavesWanted = 3200, kStep = 1024, kJoined = 16 * 64;   // kJoined: k of logprob_join_kernel
+// Waves that have places at the same time in the form with alternatives (2000 rows of 100000 in two pieces take 116 us, in three pieces, a
+// round and a bit, 133).  Pieces are whole steps (64 rows of 131072, 20 alternatives: 17.0 us in 64 pieces of two steps, 19.0 in 50 of two
+// and a half), and with alternatives there are no more than the join's registers hold (one row of 131071, 20 alternatives: 10.2 us in 128
+// pieces, 13.0 in 51, 15.1 in 33, 20.9 in 17).
+constexpr size_t kPlaces = 5120, kStep = 1024;
 // Up to here a row is not cut: 2000 scores take 5.6 us as one and 8.7 as two pieces and their join, 4000 8.3 and 8.7, 6000 9.9 and 9.0.
 constexpr size_t kWhole = 4096;
 inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
@@ -607,11 +632,11 @@ inline LogprobPlan logprob_plan(size_t n, size_t c, int top)
         p.each = (int)((c + 63) / 64);
         return p;
     }
-    // pieces while the rows alone are too few waves
-    size_t pieces = std::min((kWavesWanted + n - 1) / std::max<size_t>(n, 1), (c + kStep - 1) / kStep);
-    if (top > 0) pieces = std::min(pieces, kJoined / (size_t)top);
-    if (c <= kWhole) pieces = 1;
-    p.piece_len = (unsigned)(((c + pieces - 1) / pieces + 7) / 8 * 8);
+    if (c <= kWhole) return p;
+    size_t pieces = std::max<size_t>(kPlaces / std::max<size_t>(n, 1), 1);
+    if (top > 0) pieces = std::min(pieces, std::max<size_t>(kJoined / (size_t)top, 128));
+    const size_t steps = (c + kStep - 1) / kStep;
+    p.piece_len = (unsigned)((steps + pieces - 1) / pieces * kStep);
     p.pieces = (unsigned)((c + p.piece_len - 1) / p.piece_len);
     if (p.pieces > 1) p.work = n * p.pieces * (size_t)top * 8 + (n * p.pieces * sizeof(LogprobPart) + 15) / 16 * 16;
     return p;

@@ -111,7 +111,7 @@ def _as_u8(buf) -> np.ndarray:
     return np.frombuffer(buf, dtype=np.uint8)
 
 
-_I8 = 3                              # int8, beside the _capi.F32 / F16 / BF16 of the C ABI
+_I8, _I32 = 3, 4                     # int8 and int32, beside the _capi.F32 / F16 / BF16 of the C ABI
 _types: dict = {}                    # torch dtype -> element type; filled when the first tensor comes (torch is imported then)
 
 
@@ -120,9 +120,6 @@ def _element_type(t) -> int:
         import torch
         _types.update({torch.float32: _capi.F32, torch.float16: _capi.F16, torch.bfloat16: _capi.BF16, torch.int8: _I8, torch.int32: _I32})
     return _types.get(t.dtype, -1)
-
-
-_I32 = 4
 
 
 def torch_stream(engine: "Engine"):
@@ -153,6 +150,7 @@ class Engine:
 
     def close(self) -> None:
         self._fin()
+        self._h = C.c_void_p()   # a call after this is refused
 
     def _chk(self, rc: int) -> int:
         if rc < 0:
@@ -463,7 +461,8 @@ class Engine:
 
     def features_device(self, d_spec, batch: int, d_features) -> None:
         """apr_features_device: the pooled rows that the CNN's own head reads, for a head of one's own."""
-        self._chk(self._lib.apr_features_device(self._h, _addr(d_spec), batch, _addr(d_features)))
+        self._chk(self._lib.apr_features_device(self._h, self._vector("d_spec", d_spec, batch * Nmels * SpectrogramFrames), batch,
+                                                self._vector("d_features", d_features, batch * self.num_features)))
 
     def infer_device(self, d_spec, batch: int, d_logits) -> None:
         self._chk(self._lib.apr_infer_device(self._h, _addr(d_spec), batch, _addr(d_logits)))
@@ -576,13 +575,15 @@ class LabelHead:
                                 work_bytes=self._work_bytes, scale=self.scale)
 
     def _arguments(self, spec, target):
+        if not self._fin.alive:
+            raise ValueError("the head is closed")
         s = np.ascontiguousarray(spec, np.float32).reshape(-1, Nmels, SpectrogramFrames)
         if target is None:
             return s, None
-        t = np.ascontiguousarray(target, np.int32)
-        if t.shape != (len(s),):
-            raise ValueError(f"target is [{len(s)}], not {t.shape}")
-        return s, t
+        t = np.asarray(target)
+        if t.shape != (len(s),) or (t.size and t.dtype.kind not in "iu"):
+            raise ValueError(f"target is [{len(s)}] whole numbers, not {t.shape} of {t.dtype}")
+        return s, np.where((t >= 0) & (t < self.labels), t, -1).astype(np.int32)   # 64-bit ones must not come round to a label
 
     def score(self, spec, target=None, top: int = 5) -> dict:
         """Prepared spectrograms [n][128][188] -> dict(entropy [n], top_label [n, top], top_logprob [n, top], and with

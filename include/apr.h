@@ -327,7 +327,7 @@ int apr_engine_num_features(const apr_engine *e);   /* 0 for a front-end-only en
  * apr_engine_stream); nothing is allocated and only kernels are launched, so a call may be captured into a graph.
  * The current device of the calling thread is left as it was.  Matrices are row-major with a row stride `ld` in elements;
  * what lies between the rows' ends is neither used nor written (rows are read in aligned units of 16 bytes, whose first and last may
- * hold some of it).  Zero rows are a no-op.
+ * hold some of it).  An output shares no memory with an input or another output, except where a call says so.  Zero rows are a no-op.
  */
 
 /*

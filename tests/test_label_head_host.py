@@ -1,6 +1,7 @@
 """CPU: refusals of the label operators (argument checks come before the engine is looked at, so they need no GPU), the checks of
 their Python side, and the oracle's gradient against differences."""
 import ctypes as C
+import weakref
 
 import numpy as np
 import pytest
@@ -93,6 +94,35 @@ def test_python_side_refuses_host_and_foreign_tensors():
         e._vector("d_scale", torch.zeros(2), 2)
     assert e._matrix("d_x", 4096, 2, 3, None) == (4096, 3, _capi.F32) and e._matrix("d_x", 4096, 2, 3, 8, _capi.BF16) == (4096, 8, _capi.BF16)
     assert e._vector("d_scale", None, 2) == 0
+
+
+def test_a_closed_engine_or_head_refuses():
+    e = object.__new__(model.Engine)
+    e._lib, e.device, e._h, e._fin = _capi.lib(), 0, 1, lambda: None      # a handle that must not be looked at
+    e.close()
+    for call_ in (lambda: e.quantize_rows_device(P, 2, 3, P, P), lambda: e.linear_i8_device(P, P, P, P, 1, 2, 3, P),
+                  lambda: e.label_logprobs_device(P, 2, 3), lambda: e.label_logprobs_backward_device(P, 2, 3, P, P, P),
+                  lambda: e.features_device(P, 1, P)):
+        with pytest.raises(model.AprError):
+            call_()
+    assert e.num_features == 0
+    with pytest.raises(ValueError, match="contiguous float32"):
+        e.features_device(torch.zeros(1, 128, 188), 2, P)
+    h = object.__new__(model.LabelHead)
+    h.labels, h._fin = 5, weakref.finalize(h, int)
+    spec = np.zeros((4, 128, 188), np.float32)
+    assert h._arguments(spec, np.array([0, 4, 5, -100]))[1].tolist() == [0, 4, -1, -1]
+    assert h._arguments(spec, np.array([0, 4, 2**32, -2**32 + 1]))[1].tolist() == [0, 4, -1, -1]
+    assert h._arguments(spec, np.array([0, 4, 2**63 + 1, 1], np.uint64))[1].tolist() == [0, 4, -1, 1]
+    assert h._arguments(spec[:0], [])[1].dtype == np.int32
+    for bad in ([0, 1], [0.0, 1.0, 2.0, 3.0], [[0, 1, 2, 3]]):
+        with pytest.raises(ValueError, match="whole numbers"):
+            h._arguments(spec, bad)
+    h.close()
+    with pytest.raises(ValueError, match="closed"):
+        h.score(spec)
+    with pytest.raises(ValueError, match="closed"):
+        h.loss(spec, [0, 0, 0, 0])
 
 
 @pytest.mark.parametrize("scale", [1.0, 0.37])

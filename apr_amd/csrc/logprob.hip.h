@@ -328,8 +328,9 @@ struct Candidates {
 //
 // Candidates for the alternatives are the scores that at least `top` lanes' best scores reach: about as many as are wanted.
 // Bound by instruction issue, so what belongs to a row and not to its scores is done by a lane for each of the wave's rows, at the end.
-// 35999 x 527 bf16 takes 12.8 us without alternatives and 22.1 with five (38 MB: 8.4 us at the rate of a copy); a row at a time 15.3 and
-// 24.4, and 100000 x 64 f32 with five 31 against 37.  Eight rows a wave are no faster, and while they leave waves unused much slower.
+// 35999 x 527 bf16 takes 12.8 us without alternatives and 20.4 with five (38 MB: 8.4 us at the rate of a copy), 100000 x 64 f32 with five
+// 30.  With one row a wave these are 3, 3 and 10 us more; eight are no faster than four, and much slower while they leave waves unused.
+// Candidates looked up by a lane each instead of picked out of all scores: 1.7 us less for the 527 labels.
 constexpr unsigned kRows = 4;
 template <typename T, int E>
 __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(LogprobArgs a)
@@ -372,15 +373,39 @@ __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(Logpr
                 if (lane == 0) s_top[wave][i_row] = r.m == kNegInf ? 0 : score_key(r.m, label);
                 continue;
             }
-            Candidates c(s_list[wave]);
             // of a few labels all may be candidates
-            c.least = a.n_labels <= 16 ? kLowest : reached_by((uint32_t)key_best ^ 0x80000000u, a.top);
-            c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
-            const unsigned long long key = c.finish(a.top, lane);
-            const int place = key_place(key, c.n, c.list, lane);
+            const float least = a.n_labels <= 16 ? kLowest : reached_by((uint32_t)key_best ^ 0x80000000u, a.top);
+            // the lanes that have a candidate; while all their scores are no more than the wave's lanes, each lane looks one of them up
+            const unsigned long long hits = __ballot(best >= least);
+            unsigned long long *list = s_list[wave], key;
+            int n;
+            if (__builtin_popcountll(hits) * E <= 64) {
+                unsigned label = lane;
+                float y = v[0];
+                if (E > 1) {
+                    if (hits >> lane & 1) list[below(hits)] = lane;
+                    __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
+                    label = lane < __builtin_popcountll(hits) * E ? lane % E * 64u + (unsigned)list[lane / E] : a.n_labels;
+                    y = label < a.n_labels ? to_f32(x[label]) : kNegInf;
+                    __builtin_amdgcn_wave_barrier();
+                }
+                const unsigned long long mask = __ballot(y >= least);
+                n = __builtin_popcountll(mask);
+                if (mask >> lane & 1) list[below(mask)] = score_key(y, label);
+                __builtin_amdgcn_wave_barrier();
+                key = lane < n ? list[lane] : 0;
+                __builtin_amdgcn_wave_barrier();
+            } else {
+                Candidates c(list);
+                c.least = least;
+                c.offer(v, a.top, lane, [&](int i) { return 64u * i + lane; }, [&](int i) { return 64u * i + lane < a.n_labels ? to_f32(x[64 * i + lane]) : kNegInf; });
+                key = c.finish(a.top, lane);
+                n = c.n;
+            }
+            const int place = key_place(key, n, list, lane);
             unsigned long long *to = s_top[wave] + i_row * a.top;
-            if (lane < c.n && place < a.top) to[place] = key;
-            if (lane >= c.n && lane < a.top) to[lane] = 0;
+            if (lane < n && place < a.top) to[place] = key;
+            if (lane >= n && lane < a.top) to[lane] = 0;
         }
         const float log_s = log_of_sum(mine.s);
         if ((unsigned)lane < rows) logprob_write(a, row0 + lane, mine, log_s, to_f32(mine_t), has_t);
@@ -405,13 +430,17 @@ __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(Logpr
 // maximum itself would be new in some lane at nearly every step.  A step's 16 terms of a lane are summed before they are added.
 // 16-byte loads begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is);
 // what does not belong to the row counts as ruled out.
-// HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us, 5.4 TB/s (141 with 20 alternatives); a workgroup per row, whose waves meet
-// three times a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 11.9 us in 64 pieces a row.
+// The alternatives are among the `top` best units of 16 bytes, by a unit's best score, equal ones by their place: whatever a score
+// outside of them is, each of them holds a better one, or an equal one in front of it.  So units are collected, two or four a step and lane
+// instead of 16 scores, and the scores of those that are left are looked at when the row is done.
+// HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us, 5.4 TB/s (122 with 20 alternatives, and 141 when each score is offered by
+// itself); a workgroup per row, whose waves meet
+// three times a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 11.1 us in 64 pieces a row.
 constexpr float kGap = 8.0f;
 
-// TOP: with alternatives, whose code takes registers (95: five waves a SIMD instead of eight).
+// TOP: with alternatives, whose code takes registers (70 to 78: six waves a SIMD instead of eight).
 template <typename T, bool TOP>
-__global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(LogprobArgs a)
+__global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(LogprobArgs a)
 {
     constexpr int V = 16 / (int)sizeof(T), U = 16 / V;
     typedef T txv __attribute__((ext_vector_type(V)));
@@ -458,8 +487,14 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
                     for (int i = 1; i < V; i++) v[q * V + i] = last && (unsigned)i >= keep ? kNegInf : v[q * V + i];
                 }
             }
+            float unit_max[U];
 #pragma unroll
-            for (int e = 0; e < 16; e++) top = fmaxf(top, v[e]);
+            for (int q = 0; q < U; q++) {
+                unit_max[q] = v[q * V];
+#pragma unroll
+                for (int e = 1; e < V; e++) unit_max[q] = fmaxf(unit_max[q], v[q * V + e]);
+                top = fmaxf(top, unit_max[q]);
+            }
             m = fmaxf(m, top);
             if (__ballot(top > ref + gap)) {
                 const float higher = fmaxf(wave_reduce(top, MaxOf()), ref), d = ref - higher, w = __builtin_amdgcn_exp2f(d * c);
@@ -479,13 +514,13 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
             u += eu;
             if (TOP) {
                 if (step == 0) best.least = reached_by(top, a.top);
-                if (__ballot(top >= best.least)) {
-                    const auto label = [&](int e) { return j0 - off + ((step * U + e / V) * 64 + lane) * V + e % V; };
-                    best.offer(v, a.top, lane, label, [&](int e) {
-                        const unsigned l = label(e);   // modulo 2^32: one before the piece is far behind it
-                        return l - j0 < j1 - j0 ? to_f32(x[l]) : kNegInf;
+                if (__ballot(top >= best.least))
+                    best.offer(unit_max, a.top, lane, [&](int q) { return (step * U + q) * 64 + lane; }, [&](int q) {
+                        float y = unit_max[0];
+#pragma unroll
+                        for (int i = 1; i < U; i++) y = q == i ? unit_max[i] : y;
+                        return y;
                     });
-                }
             }
 #pragma unroll
             for (int q = 0; q < U; q++) cur[q] = next[q];
@@ -507,13 +542,29 @@ __global__ __launch_bounds__(256, TOP ? 5 : 8) void logprob_stream_kernel(Logpro
                 a.part[work] = r;
         }
         if (!TOP) continue;
-        const unsigned long long key = best.finish(a.top, lane);
+        // the best units, a lane each, once more: their scores are the candidates
+        const unsigned long long unit_key = best.finish(a.top, lane);
+        const bool has_unit = lane < best.n;
+        const unsigned first = has_unit ? (unsigned)key_label(unit_key) * V : 0;   // of the unit's scores, from the piece's first unit on
+        txv unit;
+        if (has_unit) unit = units[first / V];
+        else unit = (T)kNegInf;
+        float y[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) y[e] = has_unit && first + e >= off && first + e < len ? to_f32(unit[e]) : kNegInf;
+        Candidates c_top(s_list[wave]);
+        c_top.least = reached_by(has_unit ? key_score(unit_key) : kNegInf, a.top);
+        c_top.offer(y, a.top, lane, [&](int e) { return j0 - off + first + e; }, [&](int e) {
+            const unsigned at = first + e;
+            return has_unit && at >= off && at < len ? to_f32(x[j0 - off + at]) : kNegInf;
+        });
+        const unsigned long long key = c_top.finish(a.top, lane);
         if (a.pieces == 1)
-            logprob_write_list(a, row, r, log_s, key, best.n, best.list, lane);
+            logprob_write_list(a, row, r, log_s, key, c_top.n, c_top.list, lane);
         else {
-            const int place = key_place(key, best.n, best.list, lane);
-            if (lane < best.n && place < a.top) a.part_top[work * a.top + place] = key;
-            if (lane >= best.n && lane < a.top) a.part_top[work * a.top + lane] = 0;
+            const int place = key_place(key, c_top.n, c_top.list, lane);
+            if (lane < c_top.n && place < a.top) a.part_top[work * a.top + place] = key;
+            if (lane >= c_top.n && lane < a.top) a.part_top[work * a.top + lane] = 0;
         }
     }
 }
@@ -618,11 +669,11 @@ struct LogprobPlan {
     unsigned pieces, piece_len;
     size_t work;   // bytes
 };
-// Waves that have places at the same time in the form with alternatives (2000 rows of 100000 in two pieces take 116 us, in three pieces, a
-// round and a bit, 133).  Pieces are whole steps (64 rows of 131072, 20 alternatives: 17.0 us in 64 pieces of two steps, 19.0 in 50 of two
-// and a half), and with alternatives there are no more than the join's registers hold (one row of 131071, 20 alternatives: 10.2 us in 128
-// pieces, 13.0 in 51, 15.1 in 33, 20.9 in 17).
-constexpr size_t kPlaces = 5120, kStep = 1024;
+// Waves that have places at the same time in the form with alternatives (2000 rows of 100000 take 93 us in three pieces, 97 in two).
+// Pieces are whole steps (64 rows of 131072, 20 alternatives: 16.4 us in 64 pieces of two steps, about 2 more in 50 of two and a half), and
+// with alternatives there are no more than the join's registers hold (one row of 131071, 20 alternatives: 10.2 us in 128 pieces, 13.0 in
+// 51, 15.1 in 33, 20.9 in 17).
+constexpr size_t kPlaces = 6144, kStep = 1024;
 // Up to here a row is not cut: 2000 scores take 5.6 us as one and 8.7 as two pieces and their join, 4000 8.3 and 8.7, 6000 9.9 and 9.0.
 constexpr size_t kWhole = 4096;
 inline LogprobPlan logprob_plan(size_t n, size_t c, int top)

@@ -107,13 +107,29 @@ void launch_rowquant(const EngineView &v, const RowQuantArgs &a)
     const auto launch = [&](auto kernel, unsigned rows, unsigned threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<unsigned long long>((a.n + rows - 1) / rows, kMostBlocks)), dim3(threads), 0, v.stream, a);
     };
-    if (units <= 64) launch(rowquant_kernel<T, 1, 1>, 4, 256);
-    else if (units <= 128) launch(rowquant_kernel<T, 1, 2>, 4, 256);
-    else if (units <= 256) launch(rowquant_kernel<T, 1, 4>, 4, 256);
-    else if (units <= 512) launch(rowquant_kernel<T, 1, 8>, 4, 256);
-    else if (units <= 1024) launch(rowquant_kernel<T, 4, 4>, 1, 256);
-    else if (units <= 2048) launch(rowquant_kernel<T, 4, 8>, 1, 256);
-    else launch(rowquant_kernel<T, 16, 8>, 1, 1024);
+    if (units <= 512) {
+        switch ((units + 63) / 64) {
+        case 1: return launch(rowquant_kernel<T, 1, 1>, 4, 256);
+        case 2: return launch(rowquant_kernel<T, 1, 2>, 4, 256);
+        case 3: return launch(rowquant_kernel<T, 1, 3>, 4, 256);
+        case 4: return launch(rowquant_kernel<T, 1, 4>, 4, 256);
+        case 5: return launch(rowquant_kernel<T, 1, 5>, 4, 256);
+        case 6: return launch(rowquant_kernel<T, 1, 6>, 4, 256);
+        case 7: return launch(rowquant_kernel<T, 1, 7>, 4, 256);
+        default: return launch(rowquant_kernel<T, 1, 8>, 4, 256);
+        }
+    }
+    if (units <= 2048) {
+        switch ((units + 255) / 256) {
+        case 3: return launch(rowquant_kernel<T, 4, 3>, 1, 256);
+        case 4: return launch(rowquant_kernel<T, 4, 4>, 1, 256);
+        case 5: return launch(rowquant_kernel<T, 4, 5>, 1, 256);
+        case 6: return launch(rowquant_kernel<T, 4, 6>, 1, 256);
+        case 7: return launch(rowquant_kernel<T, 4, 7>, 1, 256);
+        default: return launch(rowquant_kernel<T, 4, 8>, 1, 256);
+        }
+    }
+    launch(rowquant_kernel<T, 16, 8>, 1, 1024);
 }
 
 // Tiles of BM x BN outputs

@@ -3,6 +3,8 @@
 // a = max |x|, scale = a / 127, q = 127 x / a rounded to nearest even.  The quotient is the exact one: t = x (127 / a) in 64 bits is
 // within 2^-45 of it, and a quotient of two 24-bit numbers that is not itself halfway between two whole numbers is at least 2^-33
 // away from there, so t rounded to a multiple of 2^-36 is on the right side, and exactly halfway where the quotient is.
+// In 32 bits x (127 / a) is within 127 * 2^-23 < 2^-16 of the quotient, so that values which are 2^-15 or more from halfway are right without
+// that; the 64 bits, an instruction of which takes twice as long, are for the waves that hold another one.
 // A row of zeros, or of nothing above 2^-119 (its scale would leave the normal range): q = 0, scale 0.  A row that holds a NaN or an
 // infinity: q = 0, scale NaN.
 #pragma once
@@ -13,7 +15,7 @@
 
 namespace apr {
 
-constexpr float kLeastRow = 0x1p-119f;
+constexpr float kLeastRow = 0x1p-119f, kToWhole = 0x1.8p+23f;   // adding kToWhole rounds to whole numbers, whose lowest 8 bits come out
 
 __device__ __forceinline__ int quantize_one(float x, double inv)
 {
@@ -32,7 +34,8 @@ struct RowQuantArgs {
 };
 
 // G waves per row, U units of 16 bytes a lane in registers, read once (a row that is longer than that is read twice).
-// HBM-bound: 35999 x 1024 f32 takes 42 us, 4.4 TB/s (a large copy: 4.7), 4096 x 8191 bf16 27 us, 3.8 TB/s.  16-byte loads
+// HBM-bound: 35999 x 1024 f32 takes 35.5 us, 5.2 TB/s (a multiplication by a number: 5.6 to 6.0), 4096 x 8191 bf16 24.3 us, 4.1 TB/s; with
+// every quotient in 64 bits 38.6 and 26.1.  16-byte loads
 // begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is); what does not belong
 // to the row counts as 0 and is not written.  A lane writes the 4 or 8 values of its unit together, at whatever alignment they have.
 template <typename T, int G, int U>
@@ -90,17 +93,32 @@ __global__ __launch_bounds__(G == 1 ? 256 : G * 64) void rowquant_kernel(RowQuan
         }
         const float am = __builtin_bit_cast(float, most);
         const bool bad = most >= 0x7F800000u, none = bad || am < kLeastRow;
-        const double inv = none ? 0.0 : 127.0 / (double)am;
+        const float inv = none ? 0.0f : 127.0f / am;
         if (me == 0) a.scale[row] = bad ? __builtin_nanf("") : none ? 0.0f : am / 127.0f;
         for (unsigned base = 0; base < n_units; base += U * LANES) {
             if (n_units > U * LANES) load(base);   // otherwise the row is still there
 #pragma unroll
             for (int i = 0; i < U; i++) {
+                asm volatile("" : "+v"(v[i]));   // or the compiler keeps what the loop above made of it, in twice the registers
+                qxv r;
+                float far = 0.0f;   // from a whole number
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float t = to_f32(v[i][e]) * inv, n = t + kToWhole;
+                    far = fmaxf(far, fabsf(t - (n - kToWhole)));
+                    r[e] = (int8_t)(uint8_t)__builtin_bit_cast(uint32_t, n);
+                }
+                if (__ballot(far > 0.5f - 0x1p-15f)) {
+                    const double exact = none ? 0.0 : 127.0 / (double)am;
+#pragma unroll
+                    for (int e = 0; e < V; e++) {
+                        r[e] = (int8_t)quantize_one(to_f32(v[i][e]), exact);
+                        __builtin_amdgcn_sched_barrier(0);   // one after the other, in few registers
+                    }
+                }
+                if (none) r = (int8_t)0;
                 const unsigned w = base + i * LANES + me;
                 if (w >= n_units) continue;
-                qxv r;
-#pragma unroll
-                for (int e = 0; e < V; e++) r[e] = none ? (int8_t)0 : (int8_t)quantize_one(to_f32(v[i][e]), inv);
                 const long long j = (long long)w * V - off;
                 if (j >= 0 && j + V <= (long long)a.k) __builtin_memcpy(q + j, &r, V);
                 else {

@@ -321,6 +321,27 @@ def test_quantize_rows(eng, k, dtype):
     assert (store[n] == 99).all() and (store[:n, k:] == 99).all() and scale[n] == GUARD
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_next_to_halves_in_every_row_length(eng, dtype):
+    # rows of every number of 16-byte units a lane, filled with the type's numbers on both sides of (j + 1/2) a / 127
+    unit = 16 // torch.empty(0, dtype=dtype).element_size()
+    for units in (50, 100, 170, 230, 300, 370, 420, 500, 700, 1000, 1200, 1500, 1700, 2000, 2300):
+        k, n = units * unit - 3, 6
+        g = torch.Generator(device=dev()).manual_seed(units)
+        a = torch.exp2(torch.tensor([0.0, 0.3, -7.7, 9.1, -13.4, 3.9], device=dev(), dtype=torch.float64)).to(dtype)
+        half = torch.randint(-127, 127, (n, k), generator=g, device=dev()).double() + 0.5
+        v = (half * a.double()[:, None] / 127).to(dtype)
+        bits = {2: torch.int16, 4: torch.int32}[v.element_size()]
+        v = (v.view(bits) + torch.randint(-1, 2, (n, k), generator=g, device=dev()).to(bits)).view(dtype)
+        v[:, k // 3] = a
+        q, s = torch.empty(n, k, device=dev(), dtype=torch.int8), torch.empty(n, device=dev())
+        torch.cuda.synchronize()
+        eng.quantize_rows_device(v, n, k, q, s)
+        eng.sync()
+        wq, ws = oracle_l.quantize(v)
+        assert torch.equal(q, wq) and torch.equal(s, ws), units
+
+
 def test_quantize_many_rows_and_odd_strides(eng):
     for n, k, ld_q in ((40000, 33, 33), (3001, 1024, 1024), (2000, 527, 529)):
         x, _ = rows(n, k, torch.float32, n)

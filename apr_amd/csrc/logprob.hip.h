@@ -328,7 +328,7 @@ struct Candidates {
 //
 // Candidates for the alternatives are the scores that at least `top` lanes' best scores reach: about as many as are wanted.
 // Bound by instruction issue, so what belongs to a row and not to its scores is done by a lane for each of the wave's rows, at the end.
-// 35999 x 527 bf16 takes 12.8 us without alternatives and 20.4 with five (38 MB: 8.4 us at the rate of a copy), 100000 x 64 f32 with five
+// 35999 x 527 bf16 takes 12.8 us without alternatives and 20.4 with five (38 MB: 6.3 us at 6 TB/s), 100000 x 64 f32 with five
 // 30.  With one row a wave these are 3, 3 and 10 us more; eight are no faster than four, and much slower while they leave waves unused.
 // Candidates looked up by a lane each instead of picked out of all scores: 1.7 us less for the 527 labels.
 constexpr unsigned kRows = 4;

@@ -188,7 +188,11 @@ extern "C" {
 size_t apr_label_logprobs_workspace(size_t n, size_t n_labels, int top)
 {
     if (n < 1 || n > kMostRows || n_labels < 1 || n_labels > kMostRows || top < 0 || top > APR_MAX_TOP) return 0;
-    return logprob_plan(n, n_labels, top).work;
+    // Without lists a row may be cut in more pieces than with them, so the most for any `top` up to this one: a call that leaves the lists
+    // out has enough with what its `top` asks for.
+    size_t work = 0;
+    for (int t = 0; t <= top; t++) work = std::max(work, logprob_plan(n, n_labels, t).work);
+    return work;
 }
 
 int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld, double scale,
@@ -209,12 +213,11 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
     if (!aligned(d_logits, element_size(dtype)) || !aligned(d_target, 4) || !aligned(d_logprob, 4) || !aligned(d_entropy, 4) || !aligned(d_stat, 4) ||
         !aligned(d_top_label, 4) || !aligned(d_top_logprob, 4))
         return refuse(e, me, "pointers are aligned to their element");
-    const size_t need = apr_label_logprobs_workspace(n, n_labels, top);
-    if (need && (!d_work || work_bytes < need || !aligned(d_work, 16))) return refuse(e, me, "d_work holds apr_label_logprobs_workspace bytes, 16-aligned");
+    const LogprobPlan plan = logprob_plan(n, n_labels, top);
+    if (plan.work && (!d_work || work_bytes < plan.work || !aligned(d_work, 16))) return refuse(e, me, "d_work holds apr_label_logprobs_workspace bytes, 16-aligned");
     LogprobArgs a;
     a.x = d_logits; a.n = n; a.ld = ld; a.n_labels = (unsigned)n_labels; a.scale = (float)scale; a.target = d_target; a.top = top;
     a.logprob = d_logprob; a.entropy = d_entropy; a.stat = d_stat; a.top_label = d_top_label; a.top_logprob = d_top_logprob;
-    const LogprobPlan plan = logprob_plan(n, n_labels, top);
     a.pieces = plan.pieces; a.piece_len = plan.piece_len;
     a.part_top = (unsigned long long *)d_work;
     a.part = (LogprobPart *)((char *)d_work + (plan.pieces > 1 ? n * plan.pieces * (size_t)top * 8 : 0));

@@ -344,8 +344,9 @@ int apr_engine_num_features(const apr_engine *e);   /* 0 for a front-end-only en
  * Any output may be NULL.  A logit of -inf rules its label out: p = 0, never an alternative; places that no label fills hold -1 and
  * -inf.  A row with every label ruled out: logprob -inf, entropy 0, stat (-inf, -inf).  A row that holds NaN or +inf: NaN everywhere,
  * top_label -1.  1 <= n_labels < 2^31, 0 <= top <= APR_MAX_TOP.
- *   d_work        scratch of apr_label_logprobs_workspace(n, n_labels, top) bytes, 16-byte aligned (0 bytes: NULL will do).  A
- *                 graph keeps its address: two calls that may run at the same time need two.
+ *   d_work        scratch of apr_label_logprobs_workspace(n, n_labels, top) bytes, 16-byte aligned (0 bytes: NULL will do).  It
+ *                 is enough for any smaller `top` and for a call without the lists, too, but not for other n.  A graph keeps its
+ *                 address: two calls that may run at the same time need two.
  */
 size_t apr_label_logprobs_workspace(size_t n, size_t n_labels, int top);
 int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld, double scale,

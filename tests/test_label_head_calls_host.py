@@ -1,0 +1,68 @@
+"""CPU: calls of the label operators that the documents allow, up to the point where they need a GPU (argument checks come before the
+engine is looked at), and what their Python side refuses."""
+import numpy as np
+import pytest
+
+from apr_amd import _capi, model
+
+P = 0x1000        # a non-null, aligned address that no call here touches
+
+
+def logprobs(n, c, top, work_bytes, lists=True):
+    """the error text of a call of those sizes without an engine"""
+    tops = (P, P) if lists else (None, None)
+    rc = _capi.lib().apr_label_logprobs_device(None, 0, P, n, c, c, 1.0, P, top, P, P, P, *tops, P, work_bytes)
+    assert rc == _capi.ERR_INVALID
+    return _capi.lib().apr_last_error(None).decode()
+
+
+LENGTHS = (1, 64, 1000, 1025, 4096, 4097, 5000, 131071, 149505, 300000, 749000, 790000, 1050000, 2885000, 3000000, 6300000, 2**31 - 1)
+
+
+def test_scratch_for_the_lists_is_enough_without_them():
+    # any output may be NULL: a call that leaves both lists out has the scratch of the `top` it names
+    for n in (1, 2, 3, 7, 48, 64, 700, 6144):
+        for c in LENGTHS:
+            for top in (0, 1, 2, 7, 8, 20, 32):
+                need = _capi.lib().apr_label_logprobs_workspace(n, c, top)
+                for lists in (True, False):
+                    why = logprobs(n, c, top, need, lists)
+                    assert why.endswith("null engine"), (n, c, top, lists, why)
+
+
+def test_scratch_does_not_fall_with_the_lists_length():
+    for n in (1, 2, 5, 60, 1000):
+        for c in LENGTHS:
+            sizes = [_capi.lib().apr_label_logprobs_workspace(n, c, top) for top in range(_capi.MAX_TOP + 1)]
+            assert sizes == sorted(sizes), (n, c, sizes)
+
+
+class Recorder:
+    """An engine's memory and sizes without a GPU"""
+    num_features = 1
+
+    def __init__(self):
+        self.sizes, self._fin = {}, type("Gone", (), {"alive": False})
+
+    def device_alloc(self, nbytes):
+        self.sizes[len(self.sizes) + 1] = nbytes
+        return len(self.sizes)
+
+    def label_logprobs_workspace(self, n, c, top):
+        return _capi.lib().apr_label_logprobs_workspace(n, c, top)
+
+    def device_upload(self, p, a):
+        pass
+
+    device_free = quantize_rows_device = sync = lambda self, *a, **k: None
+
+
+@pytest.mark.parametrize("labels,max_rows", [(2885000, 1), (3100000, 2), (800000, 3), (5000, 64), (527, 8)])
+def test_a_heads_scratch_is_enough_for_every_pass(labels, max_rows):
+    e = Recorder()
+    head = model.LabelHead(e, np.zeros((labels, 1), np.float32), max_rows=max_rows)
+    have = e.sizes[head._work] if head._work else 0
+    assert have == head._work_bytes
+    for n in range(1, max_rows + 1):
+        for top in (0, 1, 5, 8, 20, 32):
+            assert logprobs(n, labels, top, have, lists=top > 0).endswith("null engine"), (n, top)

@@ -412,6 +412,8 @@ class Engine:
         """apr_label_logprobs_device: log probability of each row's label, entropy, the `top` best labels with theirs."""
         x, ld, code = self._matrix("d_logits", d_logits, n, n_labels, ld, dtype)
         work = d_work
+        if work_bytes is not None and work_bytes < 0:    # an unsigned size in the C ABI: it would come round to a large one
+            raise ValueError(f"work_bytes is {work_bytes}")
         if d_work is None or isinstance(d_work, int):
             work, work_bytes = work or 0, work_bytes or 0
         else:

@@ -66,3 +66,49 @@ def test_a_heads_scratch_is_enough_for_every_pass(labels, max_rows):
     for n in range(1, max_rows + 1):
         for top in (0, 1, 5, 8, 20, 32):
             assert logprobs(n, labels, top, have, lists=top > 0).endswith("null engine"), (n, top)
+
+
+def no_engine():
+    """An engine's Python side without a GPU: a call that passes its checks ends as 'null engine'"""
+    e = object.__new__(model.Engine)
+    e._lib, e.device, e._h = _capi.lib(), 0, None
+    return e
+
+
+class OnGpu:
+    """What the checks ask of a tensor on GPU 0"""
+    dtype = None
+
+    def __init__(self, count):
+        self.count = count
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def numel(self):
+        return self.count
+
+    def element_size(self):
+        return 1
+
+    def data_ptr(self):
+        return P
+
+
+def test_scratch_of_a_size_that_is_none_is_refused():
+    # a negative size must not come round to a large one
+    e = no_engine()
+    need = e.label_logprobs_workspace(1, 131071, 20)
+    lists = dict(d_top_label=P, d_top_logprob=P, top=20)
+    for work, size in ((P, -1), (P, -(2**63)), (OnGpu(16), -1), (OnGpu(need), -need)):
+        with pytest.raises(ValueError, match="work_bytes"):
+            e.label_logprobs_device(P, 1, 131071, d_work=work, work_bytes=size, **lists)
+    for work, size in ((P, need - 1), (P, 0), (P, None), (OnGpu(need - 1), None), (OnGpu(need - 1), need), (OnGpu(need), need - 1), (None, None)):
+        with pytest.raises(model.AprError, match="apr_label_logprobs_workspace"):
+            e.label_logprobs_device(P, 1, 131071, d_work=work, work_bytes=size, **lists)
+    for work, size in ((P, need), (OnGpu(need), None), (OnGpu(need), need + 5)):
+        with pytest.raises(model.AprError, match="null engine"):
+            e.label_logprobs_device(P, 1, 131071, d_work=work, work_bytes=size, **lists)

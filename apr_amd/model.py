@@ -124,10 +124,12 @@ def _element_type(t) -> int:
 
 def torch_stream(engine: "Engine"):
     """The engine's stream for torch: work queued under ``torch.cuda.stream(torch_stream(engine))`` runs in order with the
-    engine's calls, so nothing has to be waited for between the two."""
+    engine's calls, so nothing has to be waited for between the two.  It ends with the engine: of a closed one there is none."""
     import torch
     s = getattr(engine, "_torch_stream", None)
     if s is None:
+        if not engine._h:     # no stream any more; address 0 would be torch's default one
+            raise AprError(_capi.ERR_INVALID, "torch_stream: the engine is closed")
         s = engine._torch_stream = torch.cuda.ExternalStream(engine._lib.apr_engine_stream(engine._h), device=engine.device)
     return s
 
@@ -151,6 +153,7 @@ class Engine:
     def close(self) -> None:
         self._fin()
         self._h = C.c_void_p()   # a call after this is refused
+        self._torch_stream = None
 
     def _chk(self, rc: int) -> int:
         if rc < 0:

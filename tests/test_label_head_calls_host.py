@@ -112,3 +112,17 @@ def test_scratch_of_a_size_that_is_none_is_refused():
     for work, size in ((P, need), (OnGpu(need), None), (OnGpu(need), need + 5)):
         with pytest.raises(model.AprError, match="null engine"):
             e.label_logprobs_device(P, 1, 131071, d_work=work, work_bytes=size, **lists)
+
+
+def test_the_stream_of_a_closed_engine_is_refused():
+    for cached in (True, False):
+        e = no_engine()
+        e._fin = lambda: None
+        if cached:
+            e._torch_stream = object()       # what an earlier torch_stream(e) kept
+            assert model.torch_stream(e) is e._torch_stream
+        e.close()
+        with pytest.raises(model.AprError, match="closed") as why:
+            model.torch_stream(e)
+        assert why.value.code == _capi.ERR_INVALID
+        e.close()                            # a second time: nothing

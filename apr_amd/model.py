@@ -504,6 +504,12 @@ def windows_in(n_bytes: int, stride: int = BytesPerSecond) -> int:
     return len(range(0, n_bytes - stride, stride))
 
 
+def _host_f32(a) -> np.ndarray:
+    if hasattr(a, "detach"):    # a tensor that trains, is on a GPU or has 16 bits is nothing that numpy takes
+        a = a.detach().float().cpu()
+    return np.ascontiguousarray(a, np.float32)
+
+
 def _release(engine: Engine, addresses: List[int]) -> None:
     while addresses:
         p = addresses.pop()
@@ -517,14 +523,14 @@ class LabelHead:
     entropy of the answer, the best alternatives.  The CNN's own head stays as it is: this one stands beside it, so that one pass of
     the convolutions serves a longer list (the reference has one head a model, at most 64 labels here).
 
-    weight [labels][features] and bias [labels] as in torch.nn.Linear; scale is 1 / temperature.  Close it before its engine."""
+    weight [labels][features] and bias [labels] as in torch.nn.Linear, arrays or tensors; scale is 1 / temperature.  Close it before its engine."""
 
     def __init__(self, engine: Engine, weight, bias=None, scale: float = 1.0, max_rows: int = 1024):
-        w = np.ascontiguousarray(weight, np.float32)
+        w = _host_f32(weight)
         f = engine.num_features
         if w.ndim != 2 or w.shape[0] < 1 or w.shape[1] != f or f == 0:
             raise ValueError(f"weight is [labels, {f}], not {w.shape}")
-        b = None if bias is None else np.ascontiguousarray(bias, np.float32)
+        b = None if bias is None else _host_f32(bias)
         if b is not None and b.shape != (w.shape[0],):
             raise ValueError(f"bias is [{w.shape[0]}], not {b.shape}")
         if max_rows < 1:

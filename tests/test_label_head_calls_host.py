@@ -2,6 +2,7 @@
 engine is looked at), and what their Python side refuses."""
 import numpy as np
 import pytest
+import torch
 
 from apr_amd import _capi, model
 
@@ -126,3 +127,22 @@ def test_the_stream_of_a_closed_engine_is_refused():
             model.torch_stream(e)
         assert why.value.code == _capi.ERR_INVALID
         e.close()                            # a second time: nothing
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.float16])
+def test_a_head_takes_the_parameters_of_a_linear(dtype):
+    # tensors that train, as torch.nn.Linear keeps them, of any type, and rows that are not one after the other
+    linear = torch.nn.Linear(1, 5).to(dtype)
+    assert linear.weight.requires_grad
+    wide = torch.randn(1, 5, dtype=dtype).t()
+    for weight in (linear.weight, wide, linear.weight.detach().float().numpy()):
+        e, up = Recorder(), []
+        e.device_upload = lambda p, a: up.append(a)
+        head = model.LabelHead(e, weight, linear.bias)
+        want = torch.as_tensor(weight).detach().float().numpy()
+        assert head.labels == 5 and all(a.dtype == np.float32 and a.flags.c_contiguous for a in up)
+        assert np.array_equal(up[0], linear.bias.detach().float().numpy()) and np.array_equal(up[1], want)
+    with pytest.raises(ValueError, match="weight"):
+        model.LabelHead(Recorder(), linear.weight[:, :0])
+    with pytest.raises(ValueError, match="bias"):
+        model.LabelHead(Recorder(), linear.weight, linear.bias[:3])

@@ -39,4 +39,25 @@ public:
     bool ok() const noexcept { return ok_; }
 };
 
+// The launches of one call.  Each returns its own error, of which the first is kept: the thread's last error (hipGetLastError) may be of
+// somebody else's earlier call, who has yet to read it.
+class Launches {
+    template <typename P>
+    struct as_is { typedef P type; };
+    hipStream_t stream_;
+    hipError_t error_ = hipSuccess;
+
+public:
+    explicit Launches(hipStream_t stream) noexcept : stream_(stream) {}
+    template <typename... P>
+    void operator()(void (*kernel)(P...), dim3 grid, dim3 block, unsigned lds, typename as_is<P>::type... p) noexcept
+    {
+        if (error_ != hipSuccess) return;
+        void *args[] = {(void *)&p...};
+        error_ = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, args, lds, stream_);
+        if (error_ != hipSuccess) (void)hipGetLastError();   // it is this call's
+    }
+    hipError_t error() const noexcept { return error_; }
+};
+
 }  // namespace apr

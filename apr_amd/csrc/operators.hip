@@ -46,10 +46,10 @@ int on_engine(apr_engine *e, const char *entry, F launch)
     }
     DeviceScope scope(v.device);
     if (!scope.ok()) return engine_fail(e, APR_ERR_DEVICE, "hipSetDevice failed");
-    launch(v);
-    const hipError_t r = hipGetLastError();
-    if (r == hipSuccess) return APR_OK;
-    snprintf(text, sizeof text, "%s: %s", entry, hipGetErrorString(r));
+    Launches go(v.stream);
+    launch(v, go);
+    if (go.error() == hipSuccess) return APR_OK;
+    snprintf(text, sizeof text, "%s: %s", entry, hipGetErrorString(go.error()));
     return engine_fail(e, APR_ERR_DEVICE, text);
 }
 
@@ -64,12 +64,12 @@ void with_type(int dtype, F f)
 #define APR_TYPE_OF(p) std::remove_pointer_t<decltype(p)>
 
 template <typename T>
-void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPlan &p)
+void launch_logprobs(const EngineView &v, Launches &go, const LogprobArgs &a, const LogprobPlan &p)
 {
     if (p.each) {
         const unsigned rows = 4 * a.rows;
         const dim3 grid((unsigned)std::min<unsigned long long>((a.n + rows - 1) / rows, kMostBlocks)), block(256);
-        const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, v.stream, a); };
+        const auto launch = [&](auto kernel) { go(kernel, grid, block, 0, a); };
         switch (p.each) {   // scores a lane: what a row has beyond them is computed for nothing
         case 1: return launch(logprob_wave_kernel<T, 1>);
         case 2: return launch(logprob_wave_kernel<T, 2>);
@@ -93,19 +93,19 @@ void launch_logprobs(const EngineView &v, const LogprobArgs &a, const LogprobPla
     const unsigned long long works = a.n * a.pieces;
     const unsigned waves = works < 4ull * v.n_cus ? 1 : 4;
     const dim3 grid((unsigned)std::min<unsigned long long>((works + waves - 1) / waves, kMostBlocks)), block(64 * waves);
-    if (a.top) hipLaunchKernelGGL((logprob_stream_kernel<T, true>), grid, block, 0, v.stream, a);
-    else hipLaunchKernelGGL((logprob_stream_kernel<T, false>), grid, block, 0, v.stream, a);
+    if (a.top) go(logprob_stream_kernel<T, true>, grid, block, 0, a);
+    else go(logprob_stream_kernel<T, false>, grid, block, 0, a);
 }
 
 // The smallest group of lanes that holds a row's 16-byte units in registers
 template <typename T>
-void launch_rowquant(const EngineView &v, const RowQuantArgs &a)
+void launch_rowquant(Launches &go, const RowQuantArgs &a)
 {
     constexpr unsigned V = 16 / sizeof(T);
     const bool whole = aligned(a.x, 16) && a.ld % V == 0;
     const unsigned long long units = (a.k + (whole ? 0ull : V - 1) + V - 1) / V;   // a row may begin inside a unit
     const auto launch = [&](auto kernel, unsigned rows, unsigned threads) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<unsigned long long>((a.n + rows - 1) / rows, kMostBlocks)), dim3(threads), 0, v.stream, a);
+        go(kernel, dim3((unsigned)std::min<unsigned long long>((a.n + rows - 1) / rows, kMostBlocks)), dim3(threads), 0, a);
     };
     if (units <= 512) {
         switch ((units + 63) / 64) {
@@ -139,14 +139,14 @@ template <int BM, int BN, int NBUF>
 constexpr int kLinearLds = (BM + BN) * 128 * NBUF;
 
 template <typename T, int BM, int BN, int NBUF, int WM, int WN, bool DMA, int EVERY>
-void launch_linear_tiles(const EngineView &v, const LinearI8Args &a)
+void launch_linear_tiles(Launches &go, const LinearI8Args &a)
 {
     const unsigned tiles_m = (a.m + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN;
-    hipLaunchKernelGGL((linear_tiles<T, BM, BN, NBUF, WM, WN, DMA, EVERY>()), dim3(tiles_m * tiles_n), dim3(WM * WN * 64), (kLinearLds<BM, BN, NBUF>), v.stream, a, tiles_m, tiles_n);
+    go(linear_tiles<T, BM, BN, NBUF, WM, WN, DMA, EVERY>(), dim3(tiles_m * tiles_n), dim3(WM * WN * 64), kLinearLds<BM, BN, NBUF>, a, tiles_m, tiles_n);
 }
 
 template <typename T>
-void launch_linear(const EngineView &v, const LinearI8Args &a)
+void launch_linear(const EngineView &v, Launches &go, const LinearI8Args &a)
 {
     const unsigned long long few = (unsigned long long)(a.m <= 16 ? 1 : (a.m + 31) / 32) * ((a.n + 15) / 16);
     const dim3 few_grid((unsigned)std::min<unsigned long long>(few, kMostBlocks));
@@ -155,15 +155,15 @@ void launch_linear(const EngineView &v, const LinearI8Args &a)
     // the tiles address their rows with 32 bits, and a grid has less than 2^32 threads
     if (a.ld_x > (1u << 22) || a.ld_w > (1u << 22) || few > (1ull << 25)) variant = kLinearFew;
     if (variant == kLinearFew) {
-        if (a.m <= 16 && whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 1, true>), few_grid, dim3(512), 0, v.stream, a);
-        else if (a.m <= 16) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 1, false>), few_grid, dim3(512), 0, v.stream, a);
-        else if (whole) hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 2, true>), few_grid, dim3(512), 0, v.stream, a);
-        else hipLaunchKernelGGL((linear_i8_few_kernel<T, 8, 2, false>), few_grid, dim3(512), 0, v.stream, a);
-    } else if (!whole) launch_linear_tiles<T, 128, 128, 2, 2, 2, false, 0>(v, a);
-    else if (variant == kLinear256) launch_linear_tiles<T, 256, 256, 2, 2, 4, true, 1>(v, a);
-    else if (variant == kLinear128) launch_linear_tiles<T, 128, 128, 2, 2, 2, true, 1>(v, a);
-    else if (variant == kLinear64Deep) launch_linear_tiles<T, 64, 64, 4, 2, 2, true, 0>(v, a);
-    else launch_linear_tiles<T, 64, 64, 2, 2, 2, true, 0>(v, a);
+        if (a.m <= 16 && whole) go(linear_i8_few_kernel<T, 8, 1, true>, few_grid, dim3(512), 0, a);
+        else if (a.m <= 16) go(linear_i8_few_kernel<T, 8, 1, false>, few_grid, dim3(512), 0, a);
+        else if (whole) go(linear_i8_few_kernel<T, 8, 2, true>, few_grid, dim3(512), 0, a);
+        else go(linear_i8_few_kernel<T, 8, 2, false>, few_grid, dim3(512), 0, a);
+    } else if (!whole) launch_linear_tiles<T, 128, 128, 2, 2, 2, false, 0>(go, a);
+    else if (variant == kLinear256) launch_linear_tiles<T, 256, 256, 2, 2, 4, true, 1>(go, a);
+    else if (variant == kLinear128) launch_linear_tiles<T, 128, 128, 2, 2, 2, true, 1>(go, a);
+    else if (variant == kLinear64Deep) launch_linear_tiles<T, 64, 64, 4, 2, 2, true, 0>(go, a);
+    else launch_linear_tiles<T, 64, 64, 2, 2, 2, true, 0>(go, a);
 }
 
 template <typename T>
@@ -208,7 +208,7 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
     if (d_logprob && !d_target) return refuse(e, me, "d_logprob needs d_target");
     if (top == 0 && (d_top_label || d_top_logprob)) d_top_label = nullptr, d_top_logprob = nullptr;
     if (!d_top_label && !d_top_logprob) top = 0;
-    if (!n) return on_engine(e, me, [](const EngineView &) {});
+    if (!n) return on_engine(e, me, [](const EngineView &, Launches &) {});
     if (!d_logits) return refuse(e, me, "null d_logits");
     if (!aligned(d_logits, element_size(dtype)) || !aligned(d_target, 4) || !aligned(d_logprob, 4) || !aligned(d_entropy, 4) || !aligned(d_stat, 4) ||
         !aligned(d_top_label, 4) || !aligned(d_top_logprob, 4))
@@ -222,11 +222,11 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
     a.part_top = (unsigned long long *)d_work;
     a.part = (LogprobPart *)((char *)d_work + (plan.pieces > 1 ? n * plan.pieces * (size_t)top * 8 : 0));
     a.per_top = top ? (65536u + top - 1) / top : 0;
-    return on_engine(e, me, [&](const EngineView &v) {
+    return on_engine(e, me, [&](const EngineView &v, Launches &go) {
         // 32 waves fit a CU: a wave takes a row until the chip is full
         a.rows = (unsigned)std::max<size_t>(1, std::min<size_t>(kRows, n / (32 * (size_t)v.n_cus)));
-        with_type(dtype, [&](auto *p) { launch_logprobs<APR_TYPE_OF(p)>(v, a, plan); });
-        if (plan.pieces > 1) hipLaunchKernelGGL(logprob_join_kernel, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(64), 0, v.stream, a, dtype);
+        with_type(dtype, [&](auto *p) { launch_logprobs<APR_TYPE_OF(p)>(v, go, a, plan); });
+        if (plan.pieces > 1) go(logprob_join_kernel, dim3((unsigned)std::min<size_t>(n, kMostBlocks)), dim3(64), 0, a, dtype);
     });
 }
 
@@ -241,7 +241,7 @@ int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_l
     if (!(scale >= kLeastScale && scale <= kMostScale)) return refuse(e, me, "1e-30 <= scale <= 1e30");
     if (d_g_logprob && !d_target) return refuse(e, me, "d_g_logprob needs d_target");
     if (d_g_entropy && !d_entropy) return refuse(e, me, "d_g_entropy needs d_entropy");
-    if (!n) return on_engine(e, me, [](const EngineView &) {});
+    if (!n) return on_engine(e, me, [](const EngineView &, Launches &) {});
     if (!d_logits || !d_stat || !d_grad) return refuse(e, me, "null d_logits, d_stat or d_grad");
     if (!aligned(d_logits, element_size(dtype)) || !aligned(d_grad, element_size(dtype)) || !aligned(d_target, 4) || !aligned(d_stat, 4) ||
         !aligned(d_entropy, 4) || !aligned(d_g_logprob, 4) || !aligned(d_g_entropy, 4))
@@ -256,11 +256,11 @@ int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_l
     const size_t units = std::max<size_t>(n_labels * element_size(dtype) / 16, 1), share = n >= kGradWaves ? units : n * units / kGradWaves;
     a.piece_units = (unsigned)std::min<size_t>(std::max<size_t>((share + 63) / 64 * 64, 64), 256);
     a.pieces = (unsigned)((units + a.piece_units - 1) / a.piece_units);
-    return on_engine(e, me, [&](const EngineView &v) {
+    return on_engine(e, me, [&](const EngineView &, Launches &go) {
         const dim3 grid((unsigned)std::min<size_t>((n * a.pieces + 3) / 4, kMostBlocks)), block(256);
         with_type(dtype, [&](auto *p) {
-            if (a.g_entropy) hipLaunchKernelGGL((logprob_grad_kernel<APR_TYPE_OF(p), true>), grid, block, 0, v.stream, a);
-            else hipLaunchKernelGGL((logprob_grad_kernel<APR_TYPE_OF(p), false>), grid, block, 0, v.stream, a);
+            if (a.g_entropy) go(logprob_grad_kernel<APR_TYPE_OF(p), true>, grid, block, 0, a);
+            else go(logprob_grad_kernel<APR_TYPE_OF(p), false>, grid, block, 0, a);
         });
     });
 }
@@ -271,13 +271,13 @@ int apr_quantize_rows_device(apr_engine *e, int dtype, const void *d_x, size_t n
     if (!dtype_ok(dtype)) return refuse(e, me, "dtype is APR_F32, APR_F16 or APR_BF16");
     if (n > kMostRows || k < 1 || k > kMostRows) return refuse(e, me, "1 <= k < 2^31, n < 2^31");
     if (ld < k || ld > kMostStride || ld_q < k || ld_q > kMostStride) return refuse(e, me, "ld and ld_q are at least k");
-    if (!n) return on_engine(e, me, [](const EngineView &) {});
+    if (!n) return on_engine(e, me, [](const EngineView &, Launches &) {});
     if (!d_x || !d_q || !d_scale) return refuse(e, me, "null pointer");
     if (!aligned(d_x, element_size(dtype)) || !aligned(d_scale, 4)) return refuse(e, me, "pointers are aligned to their element");
     RowQuantArgs a;
     a.x = d_x; a.q = d_q; a.scale = d_scale; a.n = n; a.ld = ld; a.ld_q = ld_q; a.k = (unsigned)k;
-    return on_engine(e, me, [&](const EngineView &v) {
-        with_type(dtype, [&](auto *p) { launch_rowquant<APR_TYPE_OF(p)>(v, a); });
+    return on_engine(e, me, [&](const EngineView &, Launches &go) {
+        with_type(dtype, [&](auto *p) { launch_rowquant<APR_TYPE_OF(p)>(go, a); });
     });
 }
 
@@ -290,15 +290,15 @@ int apr_linear_i8_device(apr_engine *e, const int8_t *d_x, size_t ld_x, const fl
     if (k < 1 || k > APR_LINEAR_MAX_K) return refuse(e, me, "1 <= k <= APR_LINEAR_MAX_K: the sum has 32 bits");
     if (ld_x < k || ld_x > kMostStride || ld_w < k || ld_w > kMostStride || ld_out < n || ld_out > kMostStride)
         return refuse(e, me, "ld_x and ld_w are at least k, ld_out at least n");
-    if (!m || !n) return on_engine(e, me, [](const EngineView &) {});
+    if (!m || !n) return on_engine(e, me, [](const EngineView &, Launches &) {});
     if (!d_x || !d_w || !d_x_scale || !d_w_scale || !d_out) return refuse(e, me, "null pointer");
     if (!aligned(d_out, element_size(dtype)) || !aligned(d_x_scale, 4) || !aligned(d_w_scale, 4) || !aligned(d_bias, 4))
         return refuse(e, me, "pointers are aligned to their element");
     LinearI8Args a;
     a.x = d_x; a.w = d_w; a.x_scale = d_x_scale; a.w_scale = d_w_scale; a.bias = d_bias; a.out = d_out;
     a.ld_x = ld_x; a.ld_w = ld_w; a.ld_out = ld_out; a.m = (unsigned)m; a.n = (unsigned)n; a.k = (unsigned)k;
-    return on_engine(e, me, [&](const EngineView &v) {
-        with_type(dtype, [&](auto *p) { launch_linear<APR_TYPE_OF(p)>(v, a); });
+    return on_engine(e, me, [&](const EngineView &v, Launches &go) {
+        with_type(dtype, [&](auto *p) { launch_linear<APR_TYPE_OF(p)>(v, go, a); });
     });
 }
 

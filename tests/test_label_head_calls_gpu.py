@@ -1,0 +1,53 @@
+"""GPU: calls of the label operators that the documents allow, beside other users of the GPU and at the ends of the numbers."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import label_oracle as oracle_l
+from apr_amd import _capi, model, weights as W
+from test_label_head_gpu import check, dev, near, rows, whole
+
+pytestmark = pytest.mark.gpu
+
+INVALID_DEVICE = 101          # hipErrorInvalidDevice
+
+
+@pytest.fixture(scope="module")
+def cnn(he_weights):
+    e = model.Engine(W.pack_blob(he_weights, 4), 0, 4)
+    yield e
+    e.close()
+
+
+class AnErrorBefore:
+    """The thread's last HIP error is somebody else's: a device that there is not.  It has to be there still afterwards."""
+
+    def __enter__(self):
+        torch.cuda.synchronize()
+        self.hip = _capi.lib()            # its dependencies' symbols are found through it
+        self.hip.hipGetLastError()
+        assert self.hip.hipSetDevice(10000) == INVALID_DEVICE and self.hip.hipPeekAtLastError() == INVALID_DEVICE
+
+    def __exit__(self, *exc):
+        left = self.hip.hipGetLastError()
+        assert exc[0] is not None or left == INVALID_DEVICE
+
+
+def test_an_error_of_somebody_else_is_not_the_operators(cnn):
+    x, t = rows(70, 9000, torch.bfloat16, 1)
+    E = lambda *s, d=torch.float32: torch.zeros(*s, device=dev(), dtype=d)   # noqa: E731
+    stat, ent, lp, tl, grad, q, s, out = E(70, 2), E(70), E(70), E(70, 3, d=torch.int32), E(70, 9000, d=torch.bfloat16), E(70, 9000, d=torch.int8), E(70), E(70, 70)
+    g = torch.full((70,), -1.0, device=dev())
+    work = E(cnn.label_logprobs_workspace(70, 9000, 3), d=torch.uint8)
+    with AnErrorBefore():
+        cnn.label_logprobs_device(x, 70, 9000, d_target=t, top=3, d_logprob=lp, d_entropy=ent, d_stat=stat, d_top_label=tl, d_work=work)
+        cnn.label_logprobs_backward_device(x, 70, 9000, t, stat, grad, d_g_logprob=g)
+        cnn.quantize_rows_device(x, 70, 9000, q, s)
+        cnn.linear_i8_device(q, s, q, s, 70, 70, 9000, out)
+        cnn.label_logprobs_device(x[:0], 0, 9000, d_target=t[:0])
+    cnn.sync()
+    o = oracle_l.logprobs(x, 1.0, t, 3)
+    near(lp, o["logprob"], o["tol_logprob"], "logprob")
+    assert torch.equal(tl, o["top_label"]) and torch.equal(q, oracle_l.quantize(x)[0]) and torch.isfinite(out).all() and grad.abs().sum() > 0

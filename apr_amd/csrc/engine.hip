@@ -107,6 +107,7 @@ constexpr size_t kGraphOut = (size_t)kGraphWindows * APR_SPEC_ELEMS * sizeof(flo
 struct apr_engine {
     int device = 0;
     hipStream_t stream = nullptr;
+    hipError_t launch_error = hipSuccess;   // the first one since launched() was asked
     std::string err;
     int n_classes = 0;
     int max_batch = 1024;
@@ -633,6 +634,20 @@ int prof_flush(apr_engine *e)
 }
 
 // ---- launches ---------------------------------------------------------------------------------
+template <typename... P>
+void launch(apr_engine *e, void (*kernel)(P...), dim3 grid, dim3 block, unsigned lds, typename apr::as_is<P>::type... p)
+{
+    const hipError_t r = apr::launch_kernel<P...>(e->stream, kernel, grid, block, lds, p...);
+    if (e->launch_error == hipSuccess) e->launch_error = r;
+}
+
+hipError_t launched(apr_engine *e)
+{
+    const hipError_t r = e->launch_error;
+    e->launch_error = hipSuccess;
+    return r;
+}
+
 // melT: the mel-power scratch of this launch pair (the engine's own d_melT, or the static array of the allocation-free entry)
 int run_frontend(apr_engine *e, int flavour, const uint8_t *d_pcm, size_t total_bytes, int n_windows, size_t stride,
                  float *d_out, float *melT = nullptr, bool timed = true)
@@ -646,14 +661,14 @@ int run_frontend(apr_engine *e, int flavour, const uint8_t *d_pcm, size_t total_
     {
         ProfScope ps(e, timed ? 0 : -1, (double)n_windows * T.n_frames * 5.0 * kNfft * 11.0 + 2.0 * T.nnz * T.n_frames * n_windows,
                      (double)n_windows * (std::min<size_t>(stride, APR_SAMPLE_SIZE) + (double)T.n_frames * kNmels * 4));
-        hipLaunchKernelGGL(stft_mel_kernel, dim3(n_windows * groups), dim3(64 * kFramesPerBlock), 0, e->stream, d_pcm, total_bytes, stride, n_windows, T, melT);
+        launch(e, stft_mel_kernel, dim3(n_windows * groups), dim3(64 * kFramesPerBlock), 0, d_pcm, total_bytes, stride, n_windows, T, melT);
     }
     {
         ProfScope ps(e, timed ? 1 : -1, 0.0, (double)n_windows * ((double)T.n_frames * kNmels * 4 + APR_SPEC_ELEMS * 4));
-        hipLaunchKernelGGL(db_norm_kernel, dim3(n_windows, few ? 6 : 1), dim3(256), 0, e->stream, melT, n_windows, T.n_frames,
+        launch(e, db_norm_kernel, dim3(n_windows, few ? 6 : 1), dim3(256), 0, melT, n_windows, T.n_frames,
                            T.librosa, d_out);
     }
-    HIPCHK(e, hipGetLastError());
+    HIPCHK(e, launched(e));
     return APR_OK;
 }
 
@@ -662,7 +677,7 @@ void launch_igemm(apr_engine *e, const Layer &L, const float *in, float *out, lo
 {
     const int tiles_n = L.cout / BN;
     const long long tiles_m = (M + BM - 1) / BM;   // M < 2^31: max_batch is capped at create
-    hipLaunchKernelGGL((conv3x3_igemm_f32<BM, BN, S>), dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0, e->stream, in,
+    launch(e, (conv3x3_igemm_f32<BM, BN, S>), dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0, in,
                        L.d_w, L.d_b, out, L.hin, L.win, L.cin, L.hout, L.wout, L.cout, (int)M, tiles_n);
 }
 
@@ -671,7 +686,7 @@ void launch_igemm_splitk(apr_engine *e, const Layer &L, const float *in, long lo
 {
     const int tiles_n = L.cout / BN;
     const long long tiles_m = (M + BM - 1) / BM;
-    hipLaunchKernelGGL((conv3x3_igemm_f32<BM, BN, S, 2>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)L.ksplit), dim3(256), 0, e->stream, in,
+    launch(e, (conv3x3_igemm_f32<BM, BN, S, 2>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)L.ksplit), dim3(256), 0, in,
                        L.d_w, L.d_b, e->d_part, L.hin, L.win, L.cin, L.hout, L.wout, L.cout, (int)M, tiles_n);
 }
 
@@ -680,7 +695,7 @@ void launch_wino_gemm(apr_engine *e, const Layer &L, long long T)
 {
     const int tiles_n = L.cout / 128;
     const long long tiles_m = (T + BM - 1) / BM;
-    hipLaunchKernelGGL((conv3x3_igemm_f32<BM, 128, 1, 1>), dim3((unsigned)(tiles_m * tiles_n), 16, (unsigned)L.wsplit), dim3(256), 0, e->stream, e->d_V,
+    launch(e, (conv3x3_igemm_f32<BM, 128, 1, 1>), dim3((unsigned)(tiles_m * tiles_n), 16, (unsigned)L.wsplit), dim3(256), 0, e->d_V,
                        L.d_u, L.d_b, e->d_M, 1, 1, L.cin, 1, 1, L.cout, (int)T, tiles_n);
 }
 
@@ -703,7 +718,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             ProfScope ps(e, L.slot, flops + 2.0 * 9.0 * 32.0 * (double)batch * L.hin * L.win,
                          4.0 * ((double)batch * L.hin * L.win + (double)M * L.cout + 9.0 * L.cin * L.cout));
             const unsigned n_tiles = (unsigned)batch * (unsigned)(tiles_x * tiles_y);   // <= 16384 * 48
-            hipLaunchKernelGGL(conv12_fused_kernel, dim3(std::min(n_tiles, 2u * (unsigned)e->n_cus)), dim3(256), C12_LDS_BYTES, e->stream, d_spec,
+            launch(e, conv12_fused_kernel, dim3(std::min(n_tiles, 2u * (unsigned)e->n_cus)), dim3(256), C12_LDS_BYTES, d_spec,
                                L0.d_w, L0.d_b, L.d_w, L.d_b, out, L.hin, L.win, L.hout, L.wout, tiles_x, tiles_y, n_tiles);
             in = out;
             continue;
@@ -714,10 +729,10 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             const long long tiles_m = (T + WF_TT - 1) / WF_TT;
             ProfScope ps(e, L.slot, 2.0 * 16.0 * (double)T * L.cin * L.cout, bytes + 4.0 * 7.0 * L.cin * L.cout);
             if (L.fused_waves == 4)
-                hipLaunchKernelGGL(wino_fused_f2, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), WF_LDS_BYTES, e->stream, in, L.d_u, L.d_b,
+                launch(e, wino_fused_f2, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), WF_LDS_BYTES, in, L.d_u, L.d_b,
                                    out, L.hin, L.win, L.cin, L.cout, L.th, L.tw, (int)T, tiles_n, wf_magic(tiles_n, L.th, L.tw, tiles_m));
             else
-                hipLaunchKernelGGL(wino_fused8_f2, dim3(wf8_grid((int)(tiles_m * tiles_n), e->n_cus)), dim3(512), WF8_LDS_BYTES, e->stream, in, L.d_u,
+                launch(e, wino_fused8_f2, dim3(wf8_grid((int)(tiles_m * tiles_n), e->n_cus)), dim3(512), WF8_LDS_BYTES, in, L.d_u,
                                    L.d_b, out, L.hin, L.win, L.cin, L.cout, L.th, L.tw, (int)T, tiles_n, wf_magic(tiles_n, L.th, L.tw, tiles_m, L.gn), (int)(tiles_m * tiles_n));
             in = out;
             continue;
@@ -733,7 +748,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             wa.th = L.th; wa.tw = L.tw; wa.T = (int)T; wa.tiles_n = tiles_n;
             wa.mg = wf_magic(tiles_n, L.th, L.tw, tiles_m, L.gn);
             const int n_units = (int)(tiles_m * tiles_n);
-            hipLaunchKernelGGL(wino_s2_fused, dim3(wf8_grid(n_units, e->n_cus)), dim3(512), WS_LDS_BYTES, e->stream, wa, n_units);
+            launch(e, wino_s2_fused, dim3(wf8_grid(n_units, e->n_cus)), dim3(512), WS_LDS_BYTES, wa, n_units);
             in = out;
             continue;
         }
@@ -745,15 +760,15 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
                              4.0 * ((double)batch * L.hin * L.win * L.cin + 9.0 * (double)T * L.cout + 16.0 * L.cin * L.cout));
                 const int tiles_n = L.cout / 128;
                 if (L.wbm_tile == 64)
-                    hipLaunchKernelGGL((conv3x3_igemm_f32<64, 128, 1, 3>), dim3((unsigned)(((T + 63) / 64) * tiles_n), 9), dim3(256), 0, e->stream, in,
+                    launch(e, (conv3x3_igemm_f32<64, 128, 1, 3>), dim3((unsigned)(((T + 63) / 64) * tiles_n), 9), dim3(256), 0, in,
                                        L.d_u, L.d_b, e->d_M, L.hin, L.win, L.cin, L.th, L.tw, L.cout, (int)T, tiles_n);
                 else
-                    hipLaunchKernelGGL((conv3x3_igemm_f32<128, 128, 1, 3>), dim3((unsigned)(((T + 127) / 128) * tiles_n), 9), dim3(256), 0, e->stream, in,
+                    launch(e, (conv3x3_igemm_f32<128, 128, 1, 3>), dim3((unsigned)(((T + 127) / 128) * tiles_n), 9), dim3(256), 0, in,
                                        L.d_u, L.d_b, e->d_M, L.hin, L.win, L.cin, L.th, L.tw, L.cout, (int)T, tiles_n);
             }
             {
                 ProfScope ps(e, L.slot_out, 0.0, 4.0 * (9.0 * T * L.cout + (double)M * L.cout));
-                hipLaunchKernelGGL(wino_s2_output, dim3((unsigned)std::min<long long>((nm + 255) / 256, 65536)), dim3(256), 0, e->stream,
+                launch(e, wino_s2_output, dim3((unsigned)std::min<long long>((nm + 255) / 256, 65536)), dim3(256), 0,
                                    e->d_M, L.d_b, out, L.hout, L.wout, L.cout, L.th, L.tw, T);
             }
             in = out;
@@ -765,9 +780,9 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
                 const long long n_blocks = ((T + W4_TT - 1) / W4_TT) * (L.cin / W4_BK);      // < 2^31: max_batch is capped at create
                 ProfScope ps(e, L.slot_in, 0.0, 4.0 * ((double)batch * L.hin * L.win * L.cin + 36.0 * T * L.cin));
                 if (36.0 * 4.0 * (double)T * L.cin > 2.0e9)
-                    hipLaunchKernelGGL(wino_input_f4p<true>, dim3((unsigned)n_blocks), dim3(256), 0, e->stream, in, e->d_V, L.hin, L.win, L.cin, L.th, L.tw, T, (int)n_blocks);
+                    launch(e, wino_input_f4p<true>, dim3((unsigned)n_blocks), dim3(256), 0, in, e->d_V, L.hin, L.win, L.cin, L.th, L.tw, T, (int)n_blocks);
                 else
-                    hipLaunchKernelGGL(wino_input_f4p<false>, dim3((unsigned)n_blocks), dim3(256), 0, e->stream, in, e->d_V, L.hin, L.win, L.cin, L.th, L.tw, T, (int)n_blocks);
+                    launch(e, wino_input_f4p<false>, dim3((unsigned)n_blocks), dim3(256), 0, in, e->d_V, L.hin, L.win, L.cin, L.th, L.tw, T, (int)n_blocks);
             }
             {
                 const int tiles_n = L.cout / W4_BN;
@@ -778,7 +793,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
                 wa.H = L.hout; wa.W = L.wout; wa.Cin = L.cin; wa.Cout = L.cout; wa.th = L.th; wa.tw = L.tw; wa.T = (int)T; wa.tiles_n = tiles_n;
                 wa.mg = wf_magic(tiles_n, L.th, L.tw, tiles_m, L.gn);
                 wa.n_units = (int)(tiles_m * tiles_n);
-                hipLaunchKernelGGL(wino4_fused_out, dim3(wf8_grid(wa.n_units, e->n_cus)), dim3(512), W4_LDS_BYTES, e->stream, wa);
+                launch(e, wino4_fused_out, dim3(wf8_grid(wa.n_units, e->n_cus)), dim3(512), W4_LDS_BYTES, wa);
             }
             in = out;
             continue;
@@ -788,22 +803,22 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             const long long nv = T * (L.cin / 4), nm = T * (L.cout / 4);
             {
                 ProfScope ps(e, L.slot_in, 0.0, 4.0 * ((double)batch * L.hin * L.win * L.cin + 36.0 * T * L.cin));
-                hipLaunchKernelGGL(wino_input_f4, dim3((unsigned)std::min<long long>((nv + 255) / 256, 65536)), dim3(256), 0, e->stream, in,
+                launch(e, wino_input_f4, dim3((unsigned)std::min<long long>((nv + 255) / 256, 65536)), dim3(256), 0, in,
                                    e->d_V, L.hin, L.win, L.cin, L.th, L.tw, T);
             }
             {
                 ProfScope ps(e, L.slot, 2.0 * 36.0 * (double)T * L.cin * L.cout, 4.0 * 36.0 * ((double)T * (L.cin + L.cout) + (double)L.cin * L.cout));
                 const int tiles_n = L.cout / 128;
                 if (L.wbm_tile == 64)
-                    hipLaunchKernelGGL((conv3x3_igemm_f32<64, 128, 1, 1>), dim3((unsigned)(((T + 63) / 64) * tiles_n), 36, 1), dim3(256), 0, e->stream, e->d_V,
+                    launch(e, (conv3x3_igemm_f32<64, 128, 1, 1>), dim3((unsigned)(((T + 63) / 64) * tiles_n), 36, 1), dim3(256), 0, e->d_V,
                                        L.d_u, L.d_b, e->d_M, 1, 1, L.cin, 1, 1, L.cout, (int)T, tiles_n);
                 else
-                    hipLaunchKernelGGL((conv3x3_igemm_f32<128, 128, 1, 1>), dim3((unsigned)(((T + 127) / 128) * tiles_n), 36, 1), dim3(256), 0, e->stream, e->d_V,
+                    launch(e, (conv3x3_igemm_f32<128, 128, 1, 1>), dim3((unsigned)(((T + 127) / 128) * tiles_n), 36, 1), dim3(256), 0, e->d_V,
                                        L.d_u, L.d_b, e->d_M, 1, 1, L.cin, 1, 1, L.cout, (int)T, tiles_n);
             }
             {
                 ProfScope ps(e, L.slot_out, 0.0, 4.0 * (36.0 * T * L.cout + (double)M * L.cout));
-                hipLaunchKernelGGL(wino_output_f4, dim3((unsigned)std::min<long long>((nm + 255) / 256, 65536)), dim3(256), 0, e->stream,
+                launch(e, wino_output_f4, dim3((unsigned)std::min<long long>((nm + 255) / 256, 65536)), dim3(256), 0,
                                    e->d_M, L.d_b, out, L.hout, L.wout, L.cout, L.th, L.tw, T);
             }
             in = out;
@@ -814,7 +829,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             const long long nv = T * (L.cin / 4), nm = T * (L.cout / 4);
             {
                 ProfScope ps(e, L.slot_in, 0.0, 4.0 * ((double)batch * L.hin * L.win * L.cin + 16.0 * T * L.cin));
-                hipLaunchKernelGGL(wino_input_f2, dim3((unsigned)std::min<long long>((nv + 255) / 256, 65536)), dim3(256), 0, e->stream, in,
+                launch(e, wino_input_f2, dim3((unsigned)std::min<long long>((nv + 255) / 256, 65536)), dim3(256), 0, in,
                                    e->d_V, L.hin, L.win, L.cin, L.th, L.tw, T);
             }
             {
@@ -824,7 +839,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             }
             {
                 ProfScope ps(e, L.slot_out, 0.0, 4.0 * (16.0 * T * L.cout + (double)M * L.cout));
-                hipLaunchKernelGGL(wino_output_f2, dim3((unsigned)std::min<long long>((nm + 255) / 256, 65536)), dim3(256), 0, e->stream,
+                launch(e, wino_output_f2, dim3((unsigned)std::min<long long>((nm + 255) / 256, 65536)), dim3(256), 0,
                                    e->d_M, L.d_b, out, L.hout, L.wout, L.cout, L.th, L.tw, T, L.wsplit);
             }
             in = out;
@@ -843,7 +858,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
             {
                 const long long n4 = M * L.cout / 4;
                 ProfScope ps(e, L.slot_out, 0.0, 4.0 * (L.ksplit + 1.0) * (double)M * L.cout);
-                hipLaunchKernelGGL(splitk_reduce_kernel, dim3((unsigned)std::min<long long>((n4 + 255) / 256, 4096)), dim3(256), 0, e->stream, e->d_part,
+                launch(e, splitk_reduce_kernel, dim3((unsigned)std::min<long long>((n4 + 255) / 256, 4096)), dim3(256), 0, e->d_part,
                                    L.d_b, out, n4, L.cout / 4, L.ksplit);
             }
             in = out;
@@ -853,7 +868,7 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
         if (l == 0) {
             const unsigned xchunks = (unsigned)(L.win + 3) / 4, n_rows = (unsigned)(M / L.win);   // M = windows * H * W < 2^31 (max_batch cap)
             const long long blocks = std::min<long long>(((long long)n_rows * xchunks + 31) / 32, 256 * 32);
-            hipLaunchKernelGGL(conv1_kernel, dim3((unsigned)blocks), dim3(256), 0, e->stream, in, L.d_w, L.d_b, out, L.hin,
+            launch(e, conv1_kernel, dim3((unsigned)blocks), dim3(256), 0, in, L.d_w, L.d_b, out, L.hin,
                                L.win, n_rows, xchunks);
         } else if (L.bn_tile == 128) {
             if (L.bm_tile == 64) {
@@ -870,14 +885,14 @@ int run_cnn(apr_engine *e, const float *d_spec, int batch, double trust, int emp
         in = out;
     }
     if (d_features) {
-        hipLaunchKernelGGL(pool_kernel, dim3(batch), dim3(256), 0, e->stream, in, e->pool_pixels, e->features, d_features);
+        launch(e, pool_kernel, dim3(batch), dim3(256), 0, in, e->pool_pixels, e->features, d_features);
     } else {
         ProfScope ps(e, e->head_slot, 2.0 * batch * e->features * e->n_classes,
                      4.0 * batch * e->pool_pixels * e->features);
-        hipLaunchKernelGGL(head_kernel, dim3(batch), dim3(256), 0, e->stream, in, e->pool_pixels, e->features, e->d_wfc,
+        launch(e, head_kernel, dim3(batch), dim3(256), 0, in, e->pool_pixels, e->features, e->d_wfc,
                            e->d_bfc, e->n_classes, trust, empty_class, d_logits, d_probs, d_label, d_match);
     }
-    HIPCHK(e, hipGetLastError());
+    HIPCHK(e, launched(e));
     return APR_OK;
 }
 
@@ -1574,9 +1589,9 @@ int apr_upsample_device(apr_engine *e, const int16_t *d_in, size_t n_in, int up,
     if ((rc = upsample_taps_to_device(e, taps, up * taps_per_phase))) return rc;
     const long long n_out = (long long)n_in * up;
     const unsigned blocks = (unsigned)std::min<long long>((n_out + 255) / 256, 256 * 16);
-    hipLaunchKernelGGL(apr::upsample_fir_kernel, dim3(blocks), dim3(256), 0, e->stream, d_in, 0LL, (long long)n_in, up, taps_per_phase,
+    launch(e, apr::upsample_fir_kernel, dim3(blocks), dim3(256), 0, d_in, 0LL, (long long)n_in, up, taps_per_phase,
                        e->d_rs_taps, d_out, 0LL, n_out);
-    HIPCHK(e, hipGetLastError());
+    HIPCHK(e, launched(e));
     HIPCHK(e, hipStreamSynchronize(e->stream));   // `taps` is the caller's host memory: the copy must be done on return
     return APR_OK;
 }
@@ -1600,9 +1615,9 @@ int apr_upsample(apr_engine *e, const int16_t *in, size_t n_in, int up, const do
         HIPCHK(e, hipMemcpyAsync(e->d_rs_in, in + lo, (hi - lo) * sizeof(int16_t), hipMemcpyHostToDevice, e->stream));
         const long long n_count = (long long)(m1 - m0) * up;
         const unsigned blocks = (unsigned)std::min<long long>((n_count + 255) / 256, 256 * 16);
-        hipLaunchKernelGGL(apr::upsample_fir_kernel, dim3(blocks), dim3(256), 0, e->stream, e->d_rs_in, (long long)lo, (long long)n_in, up,
+        launch(e, apr::upsample_fir_kernel, dim3(blocks), dim3(256), 0, e->d_rs_in, (long long)lo, (long long)n_in, up,
                            taps_per_phase, e->d_rs_taps, e->d_rs_out, (long long)m0 * up, n_count);
-        HIPCHK(e, hipGetLastError());
+        HIPCHK(e, launched(e));
         HIPCHK(e, hipMemcpyAsync(out + m0 * (size_t)up, e->d_rs_out, (size_t)n_count * sizeof(int16_t), hipMemcpyDeviceToHost, e->stream));
         HIPCHK(e, hipStreamSynchronize(e->stream));
     }
@@ -1621,9 +1636,9 @@ int apr_bucket_hits_device(apr_engine *e, const int32_t *d_label, const uint8_t 
     if (!n_windows) return APR_OK;
     const unsigned long long nb = (n_windows + windows_per_bucket - 1) / windows_per_bucket;
     const unsigned blocks = (unsigned)std::min<unsigned long long>((nb + 3) / 4, 256 * 8);   // one wave per bucket, grid-stride beyond that
-    hipLaunchKernelGGL(apr::bucket_hits_kernel, dim3(blocks), dim3(256), 0, e->stream, d_label, d_match, (unsigned long long)n_windows, n_classes,
+    launch(e, apr::bucket_hits_kernel, dim3(blocks), dim3(256), 0, d_label, d_match, (unsigned long long)n_windows, n_classes,
                        (unsigned long long)windows_per_bucket, nb, d_hits);
-    HIPCHK(e, hipGetLastError());
+    HIPCHK(e, launched(e));
     return APR_OK;
 }
 
@@ -2050,10 +2065,10 @@ int apr_mfma_probe(apr_engine *e, double *tflops)
     double best = 0.0;
     for (int r = 0; r < 3; r++) {                              // the first round also warms the clock up
         (void)hipEventRecord(a, e->stream);
-        hipLaunchKernelGGL(mfma_probe_kernel, dim3(blocks), dim3(256), 0, e->stream, e->d_probe, iters);
+        launch(e, mfma_probe_kernel, dim3(blocks), dim3(256), 0, e->d_probe, iters);
         (void)hipEventRecord(b, e->stream);
         float ms = 0.0f;
-        if (hipEventSynchronize(b) != hipSuccess || hipEventElapsedTime(&ms, a, b) != hipSuccess || ms <= 0.0f) {
+        if (launched(e) != hipSuccess || hipEventSynchronize(b) != hipSuccess || hipEventElapsedTime(&ms, a, b) != hipSuccess || ms <= 0.0f) {
             (void)hipEventDestroy(a); (void)hipEventDestroy(b);
             e->err = "apr_mfma_probe: launch failed";
             return APR_ERR_DEVICE;

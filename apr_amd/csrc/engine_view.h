@@ -39,11 +39,21 @@ public:
     bool ok() const noexcept { return ok_; }
 };
 
-// The launches of one call.  Each returns its own error, of which the first is kept: the thread's last error (hipGetLastError) may be of
-// somebody else's earlier call, who has yet to read it.
+// A kernel's launch, with its own error: the thread's last error (hipGetLastError) may be of somebody else's earlier call, who has yet to
+// read it.
+template <typename P>
+struct as_is { typedef P type; };
+template <typename... P>
+hipError_t launch_kernel(hipStream_t stream, void (*kernel)(P...), dim3 grid, dim3 block, unsigned lds, typename as_is<P>::type... p) noexcept
+{
+    void *args[] = {(void *)&p...};
+    const hipError_t r = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, args, lds, stream);
+    if (r != hipSuccess) (void)hipGetLastError();   // this one is reported here
+    return r;
+}
+
+// The launches of one call, up to the first error
 class Launches {
-    template <typename P>
-    struct as_is { typedef P type; };
     hipStream_t stream_;
     hipError_t error_ = hipSuccess;
 
@@ -52,10 +62,7 @@ public:
     template <typename... P>
     void operator()(void (*kernel)(P...), dim3 grid, dim3 block, unsigned lds, typename as_is<P>::type... p) noexcept
     {
-        if (error_ != hipSuccess) return;
-        void *args[] = {(void *)&p...};
-        error_ = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, args, lds, stream_);
-        if (error_ != hipSuccess) (void)hipGetLastError();   // it is this call's
+        if (error_ == hipSuccess) error_ = launch_kernel<P...>(stream_, kernel, grid, block, lds, p...);
     }
     hipError_t error() const noexcept { return error_; }
 };

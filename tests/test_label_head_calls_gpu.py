@@ -51,3 +51,33 @@ def test_an_error_of_somebody_else_is_not_the_operators(cnn):
     o = oracle_l.logprobs(x, 1.0, t, 3)
     near(lp, o["logprob"], o["tol_logprob"], "logprob")
     assert torch.equal(tl, o["top_label"]) and torch.equal(q, oracle_l.quantize(x)[0]) and torch.isfinite(out).all() and grad.abs().sum() > 0
+
+
+def test_an_error_of_somebody_else_is_not_the_engines(cnn, clips):
+    # the engine's other entry points: the same answers with it as without it
+    pcm = clips["test_bigdog"]
+    host = cnn.prepare_batch(pcm, 1, stride=192000)
+    spec = torch.from_numpy(host).to(dev())
+    f, z, hits = torch.zeros(1, 1024, device=dev()), torch.zeros(1, 4, device=dev()), torch.zeros(1, 4, device=dev(), dtype=torch.uint8)
+    label, match = torch.tensor([2], device=dev(), dtype=torch.int32), torch.tensor([1], device=dev(), dtype=torch.uint8)
+    taps = np.ones(2 * 4)
+    up_in = np.arange(50, dtype=np.int16)
+
+    def calls():
+        f.zero_(), z.zero_(), hits.zero_()
+        torch.cuda.synchronize()
+        up_out = np.zeros(100, np.int16)
+        with AnErrorBefore() if foreign else torch.no_grad():
+            cnn.features_device(spec, 1, f)
+            cnn.infer_device(spec, 1, z)
+            cnn.bucket_hits_device(label, match, 1, 4, hits, 1)
+            scored = [cnn.score(pcm, 1, 192000), cnn.classify(host), cnn.prepare(pcm)[0]]
+            assert _capi.lib().apr_upsample(cnn._h, up_in.ctypes.data, 50, 2, taps.ctypes.data, 4, up_out.ctypes.data) == 0
+        cnn.sync()
+        return [f.cpu().numpy(), z.cpu().numpy(), hits.cpu().numpy(), up_out, scored[2]] + [v for s in scored[:2] for v in s.values()]
+
+    foreign = False
+    want = calls()
+    foreign = True
+    got = calls()
+    assert all(np.array_equal(a, b) for a, b in zip(got, want)) and want[0].any() and want[1].any() and want[2].any()

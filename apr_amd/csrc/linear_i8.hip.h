@@ -39,6 +39,15 @@ __device__ __forceinline__ i32x4 linear_unit(const int8_t *row, unsigned k, unsi
     return v;
 }
 
+// The sum times both scales, one after the other.  The larger one is last where 2^31 of it are beyond the largest float (the product itself
+// then is only if the other one is as large); a whole number of the smaller one loses nothing below the normal range.
+__device__ __forceinline__ bool linear_large(float x_scale) { return fabsf(x_scale) >= 0x1p+97f; }
+__device__ __forceinline__ float linear_scaled(int sum, float x_scale, float w_scale)
+{
+    const bool large = linear_large(x_scale);
+    return (float)sum * (large ? w_scale : x_scale) * (large ? x_scale : w_scale);
+}
+
 // ---- tiled kernel: operands 16 bytes at a time, straight from memory to LDS ----
 //
 // A stage is 128 bytes of k of every row of the tile, eight units of 16 bytes; unit c of row r lies at place c ^ ((r >> 1) & 7).  An LDS
@@ -265,16 +274,21 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
     for (int i = 0; i < FM; i++) {
         const unsigned mr = wm + 32 * i;
         const float xs = mr + r32 < m_left ? a.x_scale[m0 + mr + r32] : 0.0f;
+        const auto put = [&](auto scaled) {
 #pragma unroll
-        for (int j = 0; j < FN; j++)
+            for (int j = 0; j < FN; j++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int c = 32 * j + 8 * g + 4 * half;
-                tx4 v;
+                for (int g = 0; g < 4; g++) {
+                    const int c = 32 * j + 8 * g + 4 * half;
+                    tx4 v;
 #pragma unroll
-                for (int q = 0; q < 4; q++) v[q] = from_f32<T>((float)acc[i][j][4 * g + q] * xs * s_ws[wn + c + q] + s_b[wn + c + q]);
-                *(tx4 *)(mine + r32 * ROW + c * (int)sizeof(T)) = v;
-            }
+                    for (int q = 0; q < 4; q++) v[q] = from_f32<T>(scaled(acc[i][j][4 * g + q], s_ws[wn + c + q]) + s_b[wn + c + q]);
+                    *(tx4 *)(mine + r32 * ROW + c * (int)sizeof(T)) = v;
+                }
+        };
+        // apart from each other: chosen for each output, the order takes 3 % more time of 4096 x 4096 x 1024 (28.5 us against 27.7)
+        if (__builtin_expect(__ballot(linear_large(xs)) != 0, 0)) put([&](int sum, float ws) { return linear_scaled(sum, xs, ws); });
+        else put([&](int sum, float ws) { return (float)sum * xs * ws; });
         __builtin_amdgcn_wave_barrier();   // the wave's LDS operations are in order
         if (units) {
 #pragma unroll
@@ -362,7 +376,7 @@ __global__ __launch_bounds__(W * 64) void linear_i8_few_kernel(LinearI8Args a)
 #pragma unroll
             for (int v = 0; v < W; v++) sum += s_part[v][e][lane];
             const unsigned m = m0 + 16 * (e >> 2) + 4 * quarter + (e & 3), n = n0 + r16;
-            if (m < a.m && n < a.n) ((T *)a.out)[m * a.ld_out + n] = from_f32<T>((float)sum * a.x_scale[m] * a.w_scale[n] + (a.bias ? a.bias[n] : 0.0f));
+            if (m < a.m && n < a.n) ((T *)a.out)[m * a.ld_out + n] = from_f32<T>(linear_scaled(sum, a.x_scale[m], a.w_scale[n]) + (a.bias ? a.bias[n] : 0.0f));
         }
     }
 }

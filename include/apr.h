@@ -373,8 +373,8 @@ int apr_quantize_rows_device(apr_engine *e, int dtype, const void *d_x, size_t n
 
 /*
  * out[i][j] = (sum_k x[i][k] * w[j][k]) * x_scale[i] * w_scale[j] + bias[j]: x [m][k], w [n][k] (the weight of torch.nn.Linear),
- * d_bias may be NULL.  The sum is exact (32-bit whole numbers), the rest is f32, rounded once to `dtype` (beyond its range:
- * infinity).  1 <= k <= APR_LINEAR_MAX_K; m, n <= APR_LINEAR_MAX_ROWS.  Any alignment and stride; x and w that are 16-byte
+ * d_bias may be NULL.  The sum is exact (32-bit whole numbers), the rest is f32, whose products stay in range where the whole
+ * product does, rounded once to `dtype` (beyond its range: infinity).  1 <= k <= APR_LINEAR_MAX_K; m, n <= APR_LINEAR_MAX_ROWS.  Any alignment and stride; x and w that are 16-byte
  * aligned with strides of a multiple of 16 are read 16 bytes at a time.
  */
 int apr_linear_i8_device(apr_engine *e, const int8_t *d_x, size_t ld_x, const float *d_x_scale, const int8_t *d_w, size_t ld_w,

@@ -81,3 +81,24 @@ def test_an_error_of_somebody_else_is_not_the_engines(cnn, clips):
     foreign = True
     got = calls()
     assert all(np.array_equal(a, b) for a, b in zip(got, want)) and want[0].any() and want[1].any() and want[2].any()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 70, 100), (10, 70, 100), (40, 70, 100), (520, 520, 1024), (1030, 1500, 129), (1500, 4100, 129), (2305, 3841, 129)])
+def test_product_of_a_large_and_a_small_scale(cnn, m, n, k):
+    # the whole sum times one scale may be beyond the largest float where the product with both is not; a scale of zero makes zeros
+    x, w = whole(m, k, -(-k // 16) * 16, 1), whole(n, k, -(-k // 16) * 16, 2)
+    x[1], w[1] = -128, -128
+    x[m - 1] = 0
+    one = torch.tensor([1.5, -0.75, 1.0, 1.25], device=dev())
+    xs = one.repeat(m)[:m] * torch.exp2((torch.arange(m, device=dev()) % 5 - 2) * 60.0)      # 2^-120 to 2^120
+    for dtype in (torch.float32, torch.bfloat16):
+        for ws in (torch.full((n,), 2.0 ** -118, device=dev()), torch.exp2((torch.arange(n, device=dev()) % 5 - 2) * 60.0), torch.zeros(n, device=dev()),
+                   torch.full((n,), 2.0 ** -140, device=dev())):
+            out = torch.empty(m, n, device=dev(), dtype=dtype)
+            b = torch.randn(n, generator=torch.Generator(device=dev()).manual_seed(1), device=dev())
+            for bias in (None, b):
+                torch.cuda.synchronize()
+                cnn.linear_i8_device(x, xs, w, ws, m, n, k, out, d_bias=bias, ld_x=x.stride(0), ld_w=w.stride(0))
+                cnn.sync()
+                want, tol = oracle_l.linear(x, xs, w, ws, bias, dtype)
+                near(out, want, tol, "product")

@@ -124,7 +124,9 @@ def _element_type(t) -> int:
 
 def torch_stream(engine: "Engine"):
     """The engine's stream for torch: work queued under ``torch.cuda.stream(torch_stream(engine))`` runs in order with the
-    engine's calls, so nothing has to be waited for between the two.  It ends with the engine: of a closed one there is none."""
+    engine's calls, so nothing has to be waited for between the two, and a tensor made there may be dropped as soon as its last call is
+    queued: torch hands its memory out again in this stream's order.  The stream ends with the engine: of a closed one there is none, and
+    tensors told of it (``record_stream``) have to be gone by then, as torch marks their end on it."""
     import torch
     s = getattr(engine, "_torch_stream", None)
     if s is None:
@@ -351,6 +353,8 @@ class Engine:
             raise AprError(rc, msg.decode())
 
     # ---- operators behind a label head (device-resident: torch tensors on this engine's GPU, or addresses) ----
+    # Calls are queued on the engine's stream.  Tensors that another stream makes have to be waited for before, and kept until the call has
+    # run (``sync``), not only until it returns: torch does not know that it uses them.
     def _matrix(self, name: str, a, rows: int, cols: int, ld: Optional[int], dtype: Optional[int] = None, types=(0, 1, 2)):
         """(address, row stride, element type) of a [rows, cols] operand.  A tensor speaks for itself and is checked; for an
         address the caller gives ``ld`` (default: cols) and ``dtype``."""

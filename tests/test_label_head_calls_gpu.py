@@ -102,3 +102,58 @@ def test_product_of_a_large_and_a_small_scale(cnn, m, n, k):
                 cnn.sync()
                 want, tol = oracle_l.linear(x, xs, w, ws, bias, dtype)
                 near(out, want, tol, "product")
+
+
+def test_the_chain_from_spectrograms_captured_and_replayed(cnn, clips):
+    # features -> 8 bits -> scores -> log probabilities in one graph, on new spectrograms each time, with eager work between the replays
+    n, c = 4, 300
+    E = lambda *s, d=torch.float32: torch.zeros(*s, device=dev(), dtype=d)   # noqa: E731
+    host = [cnn.prepare_batch(np.concatenate([clips[k] for k in order]), n, stride=192000)
+            for order in (sorted(clips), sorted(clips)[::-1], sorted(clips)[2:] + sorted(clips)[:2])]
+    gen = torch.Generator(device=dev()).manual_seed(1)
+    w, ws = torch.randint(-127, 128, (c, 1024), generator=gen, device=dev(), dtype=torch.int16).to(torch.int8), torch.rand(c, generator=gen, device=dev()) * 0.01
+    spec, f, q, qs, z, ent, tl = E(n, 128, 188), E(n, 1024), E(n, 1024, d=torch.int8), E(n), E(n, c), E(n), E(n, 5, d=torch.int32)
+    outs = (f, q, qs, z, ent, tl)
+
+    def calls():
+        cnn.features_device(spec, n, f)
+        cnn.quantize_rows_device(f, n, 1024, q, qs)
+        cnn.linear_i8_device(q, qs, w, ws, n, c, 1024, z)
+        cnn.label_logprobs_device(z, n, c, top=5, d_entropy=ent, d_top_label=tl)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=model.torch_stream(cnn)):
+        calls()
+    for k in range(4):
+        spec.copy_(torch.from_numpy(host[k % 3]))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for t in outs:
+            t.zero_()
+        torch.cuda.synchronize()
+        calls()
+        cnn.sync()
+        assert all(torch.equal(a, b) for a, b in zip(got, outs)) and f.any() and ent.all()
+
+
+def test_a_tensor_of_the_engines_stream_dropped_while_its_call_waits(cnn):
+    # made under the engine's stream and dropped behind the call: torch hands its memory out again in that stream's order
+    n, c = 512, 3000
+    x, t = rows(n, c, torch.float32, 1)
+    x = x.contiguous()
+    lp = torch.zeros(n, device=dev())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(model.torch_stream(cnn)):
+        y = x * 2.0
+        torch.cuda._sleep(1_000_000)              # the call waits behind it
+        cnn.label_logprobs_device(y, n, c, d_target=t, d_logprob=lp)
+        place = y.data_ptr()
+        del y
+        other = torch.full_like(x, 7.0)
+    cnn.sync()
+    assert other.data_ptr() == place              # the same memory
+    o = oracle_l.logprobs(x * 2.0, 1.0, t)
+    near(lp, o["logprob"], o["tol_logprob"], "logprob")

@@ -618,9 +618,11 @@ class LabelHead:
         return out
 
     def loss(self, spec, target) -> dict:
-        """Cross entropy of the labels, averaged over the windows that have one (0 <= target < labels), with what a training step
-        of the head needs -> dict(loss, d_logits [n, labels], features [n, features]): the weight's gradient is
-        d_logits.T @ features, the bias's d_logits.sum(0)."""
+        """Cross entropy of the labels, averaged over the windows that have one (0 <= target < labels), with what a step of a
+        training loop outside needs -> dict(loss, d_logits [n, labels], features [n, features]).  d_logits is the gradient of this loss,
+        and d_logits.sum(0) the bias's.  d_logits.T @ features is an estimate for a 32-bit weight, not that gradient: it takes the
+        rounding to 8 bits of both operands as the identity (straight through), and the features as they were before it.  A head's own
+        weight stays what it was made of: a new one is a new head."""
         s, t = self._arguments(spec, target)
         if t is None:
             raise ValueError("a loss needs targets")

@@ -57,7 +57,7 @@ __device__ __forceinline__ float linear_scaled(int sum, float x_scale, float w_s
 // A DMA instruction fills 1 KiB of LDS, eight rows, lane by lane; the swizzle is which unit each lane asks for.  Rows past the matrix
 // and units past k are out of the buffer's range, which reads as 0.
 //
-// What bounds 256 x 256 tiles: the chip's power.  16384 x 8192 x 8192 takes 0.92-0.95 ms (2.3-2.4 POPS) at 1.8 GHz, where the matrix units work
+// What bounds 256 x 256 tiles: the chip's power.  16384 x 8192 x 8192 takes 0.92 ms a call among others (2.4 POPS; 0.94-0.97 by the profiler) at 1.8 GHz, where the matrix units work
 // 62 % of the cycles; matrix instructions alone, without loads, take 0.69 ms, since random operands bring the clock down (from
 // registers 3.1-3.5 POPS, and 4.6 on zeros), and with the LDS reads 0.78.
 // LDS-DMA: 64 lanes x 16 B from a buffer to 1 KiB of LDS at byte address lds (wave-uniform).  The caller waits on vmcnt.
@@ -387,8 +387,8 @@ __global__ __launch_bounds__(W * 64) void linear_i8_few_kernel(LinearI8Args a)
 // shared by the `beside` tiles that fit a CU together) or `full` for each tile (its throughput), whichever is longer.  Measured with
 // one to eight rounds of tiles, bf16 out; 1024 x 8192 x 8192: 98 / 73 / 121 / 103 us by 256 x 256, 128 x 128, 64 x 64 with four and with
 // two stages (the rule: 98 / 73 / 127 / 105), 256 x 8192 x 8192: 85 / 50 / 32 / 39 (98 / 50 / 34 / 39), 16384 x 8192 x 8192: 925 / 1113 / 1780 / 1612.
-// The few kernel: 2.3 us and, for each tile of a CU, 0.8 ns a k (16 m) or 1.4 ns a k (32 m): 256 x 527 x 1024 takes 5.1 us against 6.7 by
-// 64 x 64 tiles, 64 x 2000 x 4096 8.7; 4096 x 527 x 1024 would take 30 against 9.4.
+// The few kernel: 2.3 us and, for each tile of a CU, 0.8 ns a k (16 m) or 1.4 ns a k (32 m): 256 x 527 x 1024 takes
+// 5.1 us in a captured row of calls (5.8 by the profiler) against 6.7 by 64 x 64 tiles, 64 x 2000 x 4096 8.7; 4096 x 527 x 1024 would take 30 against 9.4.
 struct LinearCost {
     int tile, beside;
     float t0, alone, full;

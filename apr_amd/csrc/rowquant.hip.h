@@ -34,8 +34,8 @@ struct RowQuantArgs {
 };
 
 // G waves per row, U units of 16 bytes a lane in registers, read once (a row that is longer than that is read twice).
-// HBM-bound: 35999 x 1024 f32 takes 35.5 us, 5.2 TB/s (a multiplication by a number: 5.6 to 6.0), 4096 x 8191 bf16 24.3 us, 4.1 TB/s; with
-// every quotient in 64 bits 38.6 and 26.1.  16-byte loads
+// HBM-bound: 35999 x 1024 f32 takes 35.2 us, 5.2 TB/s (a multiplication by a number: 5.6 to 6.0), 4096 x 8191 bf16 25.8 us, 3.9 TB/s; in a
+// captured row of calls 35.5 and 24.3, and with every quotient in 64 bits 38.6 and 26.1.  16-byte loads
 // begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is); what does not belong
 // to the row counts as 0 and is not written.  A lane writes the 4 or 8 values of its unit together, at whatever alignment they have.
 template <typename T, int G, int U>

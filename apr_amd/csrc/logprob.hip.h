@@ -425,9 +425,11 @@ __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(Logpr
 
 // ---- longer rows: a wave per row, or per piece of one, 1024 scores at a time, the next ones on their way ----
 //
-// No lane waits for another wave.  The sums are relative to a reference that the wave shares: the best score so far, renewed only
-// when a score passes it by more than kGap (then exp <= e^kGap, and nothing is lost: the sums are floating point), because the running
-// maximum itself would be new in some lane at nearly every step.  A step's 16 terms of a lane are summed before they are added.
+// No lane waits for another wave.  The sums are relative to the best score so far, which the wave shares: it is new in the k-th of many
+// steps once in k times or so, where a lane's own maximum would be new in some lane at nearly every step.  It is renewed for any better score:
+// relative to one that is g lower, s and u hold terms up to e^(scale g) and g e^(scale g), and what is left of their roundings when u is
+// moved to the maximum, scale g times that of s, is too much for the entropy of a nearly sure answer (off by 3e-6 with g of up to
+// 8 / scale).  A step's 16 terms of a lane are summed before they are added.
 // 16-byte loads begin at the 16-byte unit that the row begins in (which is inside the allocation, as the row's first element is);
 // what does not belong to the row counts as ruled out.
 // The alternatives are among the `top` best units of 16 bytes, by a unit's best score, equal ones by their place: whatever a score
@@ -436,9 +438,7 @@ __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(Logpr
 // HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us a call among others, 5.5 TB/s (95 to 100 by the
 // profiler; 120 with 20 alternatives, and 141 when each score is offered by itself); a workgroup per row, whose waves meet three times
 // a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 11.2 us in 64 pieces a row.
-constexpr float kGap = 8.0f;
-
-// TOP: with alternatives, whose code takes registers (70 to 78: six waves a SIMD instead of eight).
+// TOP: with alternatives, whose code takes registers (68 to 77: six or seven waves a SIMD instead of eight).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(LogprobArgs a)
 {
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(Logpro
     __shared__ __align__(16) unsigned long long s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const unsigned long long works = a.n * a.pieces;
-    const float c = a.scale * kLog2E, gap = kGap / a.scale, least_t = -200.0f / a.scale;
+    const float c = a.scale * kLog2E, least_t = -200.0f / a.scale;
     for (unsigned long long work = (unsigned long long)blockIdx.x * waves + wave; work < works; work += (unsigned long long)gridDim.x * waves) {
         const unsigned long long row = a.pieces == 1 ? work : work / a.pieces;
         const unsigned piece = (unsigned)(work - row * a.pieces);
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(Logpro
             }
         };
         load(cur, 0);
-        float m = kNegInf, ref = kNegInf, s = 0.0f, u = 0.0f;
+        float m = kNegInf, s = 0.0f, u = 0.0f;   // m: wave-uniform
         Candidates best(s_list[wave]);
         for (unsigned step = 0; step < steps; step++) {
             if (step + 1 < steps) load(next, step + 1);
@@ -495,14 +495,13 @@ __global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(Logpro
                 for (int e = 1; e < V; e++) unit_max[q] = fmaxf(unit_max[q], v[q * V + e]);
                 top = fmaxf(top, unit_max[q]);
             }
-            m = fmaxf(m, top);
-            if (__ballot(top > ref + gap)) {
-                const float higher = fmaxf(wave_reduce(top, MaxOf()), ref), d = ref - higher, w = __builtin_amdgcn_exp2f(d * c);
+            if (__ballot(top > m)) {
+                const float higher = wave_reduce(top, MaxOf()), d = m - higher, w = __builtin_amdgcn_exp2f(d * c);
                 u = w * fmaf(fmaxf(d, least_t), s, u);
                 s *= w;
-                ref = higher;
+                m = higher;
             }
-            const float r = ref == kNegInf ? 0.0f : ref;
+            const float r = m == kNegInf ? 0.0f : m;
             float es = 0.0f, eu = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -526,12 +525,10 @@ __global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(Logpro
             for (int q = 0; q < U; q++) cur[q] = next[q];
         }
         LogprobPart r;
-        r.m = wave_reduce(m, MaxOf());
-        // a reference of -inf: every score ruled out, or NaN in s
-        const float d = ref == kNegInf ? 0.0f : ref - r.m, w = __builtin_amdgcn_exp2f(d * c);
         wave_sums(s, u);
-        r.s = w * s;
-        r.u = w * fmaf(fmaxf(d, least_t), s, u);
+        r.m = m;
+        r.s = s;
+        r.u = u;
         const float log_s = log_of_sum(r.s);
         if (lane == 0) {
             if (a.pieces == 1) {

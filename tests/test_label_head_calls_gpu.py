@@ -157,3 +157,18 @@ def test_a_tensor_of_the_engines_stream_dropped_while_its_call_waits(cnn):
     assert other.data_ptr() == place              # the same memory
     o = oracle_l.logprobs(x * 2.0, 1.0, t)
     near(lp, o["logprob"], o["tol_logprob"], "logprob")
+
+
+@pytest.mark.parametrize("c", [1100, 1239, 4000, 20000])
+@pytest.mark.parametrize("scale", [1.0, 7.0])
+def test_a_best_score_behind_one_that_is_nearly_as_good(cnn, c, scale):
+    # a first part of the row with a maximum of its own, then the row's, up to 8 nats higher: the sums stay relative to the largest score,
+    # so that the entropy of an answer that is nearly sure is as exact as any
+    n = 3000
+    gen = torch.Generator(device=dev()).manual_seed(c)
+    x = torch.rand(n, c, generator=gen, device=dev()) * 2 - 5
+    x[:, 1000] = 0.0
+    at = torch.randint(1060, c, (n,), generator=gen, device=dev())
+    x.scatter_(1, at[:, None], 6.0 + 2 * torch.rand(n, 1, generator=gen, device=dev()))
+    for dtype in (torch.float32, torch.bfloat16):
+        check(cnn, (x / scale).to(dtype), at.int(), top=2, scale=scale)

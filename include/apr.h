@@ -357,7 +357,9 @@ int apr_label_logprobs_device(apr_engine *e, int dtype, const void *d_logits, si
  * Gradient of sum_i g_logprob[i] * logprob[i] + g_entropy[i] * entropy[i] with respect to the logits, in the logits' type (one
  * rounding).  d_stat and d_entropy are what the forward call wrote for these logits and this scale.  d_g_logprob (needs d_target)
  * or d_g_entropy (needs d_entropy) may be NULL: zero.  Cross entropy averaged over n rows: g_logprob = -1 / n.  A target outside
- * [0, n_labels) has no gradient, a row with every label ruled out neither; a row of NaN gives NaN.  d_grad may be d_logits.
+ * [0, n_labels) has no gradient, a row with every label ruled out neither; a row of NaN gives NaN.  A probability below 2^-126
+ * counts as 0, and scale * g_logprob and scale * g_entropy are held as floats: beyond their range the gradient is infinite or NaN.
+ * d_grad may be d_logits.
  */
 int apr_label_logprobs_backward_device(apr_engine *e, int dtype, const void *d_logits, size_t n, size_t n_labels, size_t ld,
                                        double scale, const int32_t *d_target, const float *d_stat, const float *d_entropy,

@@ -585,7 +585,7 @@ __global__ __launch_bounds__(256) void head_kernel(const float *__restrict__ act
 }
 
 // The first half of head_kernel: act [B][P][F] -> max over P -> feat [B][F].  One workgroup per window.
-// 1024 windows take 9.6 us, 4 take 6.5: next to nothing beside the convolutions.
+// 1024 windows take 9.7 us, 4 take 6.4: next to nothing beside the convolutions.
 __global__ __launch_bounds__(256) void pool_kernel(const float *__restrict__ act, int P, int F, float *__restrict__ feat)
 {
     const long long win = blockIdx.x;

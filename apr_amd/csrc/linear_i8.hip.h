@@ -57,9 +57,9 @@ __device__ __forceinline__ float linear_scaled(int sum, float x_scale, float w_s
 // A DMA instruction fills 1 KiB of LDS, eight rows, lane by lane; the swizzle is which unit each lane asks for.  Rows past the matrix
 // and units past k are out of the buffer's range, which reads as 0.
 //
-// What bounds 256 x 256 tiles: the chip's power.  16384 x 8192 x 8192 takes 0.92 ms a call among others (2.4 POPS; 0.94-0.97 by the profiler) at 1.8 GHz, where the matrix units work
-// 62 % of the cycles; matrix instructions alone, without loads, take 0.69 ms, since random operands bring the clock down (from
-// registers 3.1-3.5 POPS, and 4.6 on zeros), and with the LDS reads 0.78.
+// What bounds 256 x 256 tiles: the chip's power.  16384 x 8192 x 8192 takes 0.92-0.94 ms a call among others (2.3-2.4 POPS;
+// 0.94-0.98 by the profiler) at 1.8 GHz, where the matrix units work 62 % of the cycles; matrix instructions alone, without loads, take
+// 0.69 ms, since random operands bring the clock down (from registers 3.1-3.5 POPS, and 4.6 on zeros), and with the LDS reads 0.78.
 // LDS-DMA: 64 lanes x 16 B from a buffer to 1 KiB of LDS at byte address lds (wave-uniform).  The caller waits on vmcnt.
 __device__ __forceinline__ void linear_dma(i32x4 rs, unsigned voff, unsigned lds)
 {
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void linear_i8_tile_kernel(LinearI
 //
 // Blocks of 256 k go to the W waves in turn.  A load takes 64 neighbouring bytes of 16 rows (the 16 x 16 x 64 instruction's layout: with the
 // 32 x 32 x 32 one a load takes 32 bytes of 32 rows, and the lines of 16 waves do not stay in the L1 until the rest is asked for:
-// 1 x 8192 x 8192 takes 14.2 us against 19.4, 4.7 TB/s of weights; twice as many loads in flight: the same).  The waves' partial sums, exact whole numbers, meet in LDS.
+// 1 x 8192 x 8192 takes 14.3 us against 19.4, 4.7 TB/s of weights; twice as many loads in flight: the same).  The waves' partial sums, exact whole numbers, meet in LDS.
 template <typename T, int W, int G, bool WHOLE>
 __global__ __launch_bounds__(W * 64) void linear_i8_few_kernel(LinearI8Args a)
 {

@@ -328,7 +328,7 @@ struct Candidates {
 //
 // Candidates for the alternatives are the scores that at least `top` lanes' best scores reach: about as many as are wanted.
 // Bound by instruction issue, so what belongs to a row and not to its scores is done by a lane for each of the wave's rows, at the end.
-// 35999 x 527 bf16 takes 13.3 us without alternatives and 20.3 with five (38 MB: 6.3 us at 6 TB/s), 100000 x 64 f32 with five
+// 35999 x 527 bf16 takes 13.2 us without alternatives and 20.6 with five (38 MB: 6.3 us at 6 TB/s), 100000 x 64 f32 with five
 // 31.  With one row a wave these are 3, 3 and 10 us more; eight are no faster than four, and much slower while they leave waves unused.
 // Candidates looked up by a lane each instead of picked out of all scores: 1.7 us less for the 527 labels.
 constexpr unsigned kRows = 4;
@@ -435,8 +435,8 @@ __global__ __launch_bounds__(256, E > 12 ? 7 : 8) void logprob_wave_kernel(Logpr
 // The alternatives are among the `top` best units of 16 bytes, by a unit's best score, equal ones by their place: whatever a score
 // outside of them is, each of them holds a better one, or an equal one in front of it.  So units are collected, two or four a step and lane
 // instead of 16 scores, and the scores of those that are left are looked at when the row is done.
-// HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us a call among others, 5.5 TB/s (95 to 100 by the
-// profiler; 120 with 20 alternatives, and 141 when each score is offered by itself); a workgroup per row, whose waves meet three times
+// HBM-bound without alternatives: 8192 x 32000 bf16 takes 96 us a call among others, 5.5 TB/s (97 to 101 by the
+// profiler; 122 with 20 alternatives, and 141 when each score is offered by itself); a workgroup per row, whose waves meet three times
 // a row, took 158.  Few rows are bound by latency: 64 x 131072 with 20 alternatives takes 11.2 us in 64 pieces a row.
 // TOP: with alternatives, whose code takes registers (68 to 77: six or seven waves a SIMD instead of eight).
 template <typename T, bool TOP>
@@ -569,7 +569,7 @@ __global__ __launch_bounds__(256, TOP ? 6 : 8) void logprob_stream_kernel(Logpro
 constexpr unsigned kJoined = 1024, kHeads = 8;
 static_assert(2 * kHeads == kJoined / 64, "one set of registers for both");
 
-// ---- the pieces of a row joined, a wave per row: 5.6 us for one row, 5.2 for 64, most of it the launch and two loads in a row ----
+// ---- the pieces of a row joined, a wave per row: 5.8 us for one row, 5.4 for 64, most of it the launch and two loads in a row ----
 __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a, int type)
 {
     __shared__ __align__(16) unsigned long long s_list[64];
